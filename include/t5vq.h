@@ -411,6 +411,64 @@ int t5vq_rmsnorm_sqnorms_img_f32(const float* hidden, const float* gamma, const 
                                  int64_t N, int64_t D, float* x_out, float* xx, float* rms, void* token_image,
                                  t5vq_stream_t stream);
 
+/* ---- Dropout from a counter, layer / RMS norm, and the sum of a residual stream with a sublayer's output ----------
+ * What stands around the encoder's last norm: the dropout and residual sum of the sublayer before it, the norm, and the
+ * dropout behind it (python_transformers/modeling_t5.py:864-865), for fp32, bf16 and fp16 rows of any length D >= 1 that start at any multiple of their element's size.  Arithmetic, statistics and
+ * sums are fp32; every output is rounded once, to nearest even.
+ *
+ * Random numbers.  No mask is stored: a kernel draws an element's 16 bits from Philox4x32-10 (Salmon et al., SC 2011)
+ * with the key `seed` and the counter (offset / 4 + site: 64 bits, col / 8: 32 bits, row: 32 bits); column 8b + j takes
+ * half j % 2 (low half first) of word j / 2.  It is kept iff those bits are below K = t5vq_dropout_keep_count(p) =
+ * round_half_even((1 - p) * 65536), and a kept value is multiplied by fp32(65536 / K), so the expectation is exact
+ * although p is rounded to a multiple of 2^-16.  A dropped value is 0 whatever it was.  K == 65536 (p < 2^-17): no
+ * dropout; K == 0: everything is dropped.
+ *   Forward calls take {seed, offset} by value, and (both nullable) from device memory: *seed_dev REPLACES seed,
+ *   *offset_dev is ADDED to offset -- a generator that a graph replays, or an earlier call's ticket.  ticket_out
+ *   (nullable) receives the {seed, offset} the call drew with; backward calls take it as `ticket`.  Site 0 is a dropout
+ *   by itself or that of the branch, site 1 that of a norm's output; a call uses offset .. offset + 7, so calls whose
+ *   offsets are 8 apart share no numbers. */
+#define T5VQ_F32 0
+#define T5VQ_BF16 1
+#define T5VQ_F16 2
+#define T5VQ_NORM_LAYER 0
+#define T5VQ_NORM_RMS 1
+
+/* K as above; -1 for p outside [0, 1]. */
+int64_t t5vq_dropout_keep_count(double p);
+
+/* y = residual + (kept ? x * scale : 0), residual nullable and of y's type; x and y are of one type, or one of them is
+ * fp32.  The gradient of x is the same call on the gradient of y, without residual, with the forward's ticket. */
+int t5vq_dropout_add(const void* x, int x_type, const void* residual, int64_t N, int64_t D, double p, int64_t seed,
+                     int64_t offset, const int64_t* seed_dev, const int64_t* offset_dev, int64_t* ticket_out, void* y,
+                     int y_type, t5vq_stream_t stream);
+
+/* h   = branch ? round(hidden + (kept ? branch * scale : 0)) : hidden          site 0; rounded to hidden's type
+ * out = kept ? ((h - mean) * r * weight + bias) * scale : 0                     site 1; bias nullable
+ *   T5VQ_NORM_LAYER: mean = mean_d h, r = 1 / sqrt(mean_d (h - mean)^2 + eps);  T5VQ_NORM_RMS: mean = 0 in both
+ *   branch (nullable): of hidden's type, or any type beside an fp32 hidden (autocast).  sum [N,D] receives h (required
+ *   with branch, unused without); out: of hidden's type, or fp32.  stats [N,2] (nullable) = {mean, r} for backward.
+ *   xx [N] and token_image (nullable; out fp32, D % 4 == 0, D <= 2048): the row norms and the fp16 image of `out` that
+ *   the searches take, bit-identical to what they would compute themselves. */
+int t5vq_norm_forward(const void* hidden, int hidden_type, const void* branch, int branch_type, const void* weight,
+                      const void* bias, int weight_type, int norm_kind, float eps, int64_t N, int64_t D, double branch_p,
+                      double p, int64_t seed, int64_t offset, const int64_t* seed_dev, const int64_t* offset_dev,
+                      int64_t* ticket_out, void* out, int out_type, void* sum, float* stats, float* xx,
+                      void* token_image, t5vq_stream_t stream);
+
+/* Autograd of the above from the normed rows h (the forward's sum, or hidden).  gy = kept ? grad_out * scale : 0,
+ * a = gy * weight, n = (h - mean) * r:
+ *   grad_hidden = r * (a - mean_d a - n * mean_d (a n)) + grad_sum      (no mean_d a for T5VQ_NORM_RMS; grad_sum nullable)
+ *   grad_branch = kept ? grad_hidden * scale : 0   (nullable; from grad_hidden before it is rounded)
+ *   grad_weight[d] = sum_i gy n,  grad_bias[d] = sum_i gy   (nullable; of weight's type; deterministic, no atomics)
+ * ticket: the forward's, null only if nothing was dropped.  Parameter gradients need a workspace of
+ * t5vq_norm_backward_workspace_bytes(N, D) bytes. */
+int64_t t5vq_norm_backward_workspace_bytes(int64_t N, int64_t D);
+int t5vq_norm_backward(const void* grad_out, int out_type, const void* grad_sum, const void* h, int hidden_type,
+                       const void* weight, int weight_type, int norm_kind, const float* stats, int64_t N, int64_t D,
+                       double branch_p, double p, const int64_t* ticket, void* grad_hidden, void* grad_branch,
+                       int branch_type, void* grad_weight, void* grad_bias, void* workspace, int64_t workspace_bytes,
+                       t5vq_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -10,7 +10,7 @@ from __future__ import annotations
 import ctypes
 import os
 import threading
-from ctypes import c_char_p, c_float, c_int, c_int64, c_void_p
+from ctypes import c_char_p, c_double, c_float, c_int, c_int64, c_void_p
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # T5VQ_LIB: another build of the same library (variant builds for A/B timing); there is still no CPU path behind it
@@ -75,6 +75,13 @@ SIGNATURES = {
                                                  P, c_int, P, P]),
     "t5vq_vq_ema_finalize_img_f32": (c_int, [P, P, P, P, P, P, I64, I64, I64, I64, c_float, c_float, c_float, c_float,
                                              c_float, c_float, c_int, c_int, P, P, P, P]),
+    "t5vq_dropout_keep_count": (I64, [c_double]),
+    "t5vq_dropout_add": (c_int, [P, c_int, P, I64, I64, c_double, I64, I64, P, P, P, P, c_int, P]),
+    "t5vq_norm_forward": (c_int, [P, c_int, P, c_int, P, P, c_int, c_int, c_float, I64, I64, c_double, c_double, I64, I64,
+                                  P, P, P, P, c_int, P, P, P, P, P]),
+    "t5vq_norm_backward_workspace_bytes": (I64, [I64, I64]),
+    "t5vq_norm_backward": (c_int, [P, c_int, P, P, c_int, P, c_int, c_int, P, I64, I64, c_double, c_double, P, P, P, c_int,
+                                   P, P, P, I64, P]),
 }
 
 TORCH_LIB_PATH = os.environ.get("T5VQ_TORCH_LIB") or os.path.join(_HERE, "csrc", "libt5vq_torch.so")
@@ -90,7 +97,7 @@ _torch_ops_error = None
 
 _load_lock = threading.RLock()
 
-ABI_VERSION = 310     # t5vq_version() of the library these signatures were written against (image-emitting _img entry points)
+ABI_VERSION = 320     # t5vq_version() of the library these signatures were written against (dropout / norm entry points)
 
 
 class T5VQError(RuntimeError):

@@ -2315,7 +2315,7 @@ int launch_dist_self(const float* x, const float* w, const float* xx, const floa
 // ================================================================================================
 extern "C" {
 
-int t5vq_version(void) { return 310; }
+int t5vq_version(void) { return 320; }
 int t5vq_set_tuning(int variant) {
     g_depth2 = variant >= 100000 ? 0 : 1;   // +100000: single staging register set
     variant %= 100000;

@@ -1,0 +1,146 @@
+// Internal to libt5vq.so: what the dropout / norm kernels share (t5vq_norm.hip, t5vq_norm_backward.hip).
+//
+// Rows are walked in GROUPS of four consecutive columns: group q = columns 4q .. 4q + 3, one group per lane.  A row of any
+// length starts at any multiple of its element's size, so group accesses promise the compiler no more than the element's
+// alignment (gfx950 reads and writes global memory at any byte address; one 16- or 8-byte access per group all the same);
+// only the last group of a row with D % 4 != 0 goes element by element.
+#ifndef T5VQ_NORM_H_
+#define T5VQ_NORM_H_
+#include "t5vq_internal.h"
+
+namespace t5vq_norm {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+
+template <class T> struct Group;   // four elements of T in memory, aligned like one
+template <> struct Group<float> { typedef float type __attribute__((ext_vector_type(4), aligned(4))); };
+template <> struct Group<__bf16> { typedef __bf16 type __attribute__((ext_vector_type(4), aligned(2))); };
+template <> struct Group<_Float16> { typedef _Float16 type __attribute__((ext_vector_type(4), aligned(2))); };
+
+// columns c .. c + 3 of a row of D elements; columns >= D read as 0
+template <class T>
+__device__ __forceinline__ f32x4 load_group(const T* __restrict__ row, int c, int D) {
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (c + 4 <= D) {
+        v = __builtin_convertvector(*reinterpret_cast<const typename Group<T>::type*>(row + c), f32x4);
+    } else if (c < D) {
+        v.x = static_cast<float>(row[c]);
+        if (c + 1 < D) v.y = static_cast<float>(row[c + 1]);
+        if (c + 2 < D) v.z = static_cast<float>(row[c + 2]);
+    }
+    return v;
+}
+// each value rounded once, to nearest even
+template <class T>
+__device__ __forceinline__ void store_group(T* __restrict__ row, int c, int D, f32x4 v) {
+    if (c + 4 <= D) {
+        typedef typename Group<T>::type G;
+        *reinterpret_cast<G*>(row + c) = __builtin_convertvector(v, G);
+    } else if (c < D) {
+        row[c] = static_cast<T>(v.x);
+        if (c + 1 < D) row[c + 1] = static_cast<T>(v.y);
+        if (c + 2 < D) row[c + 2] = static_cast<T>(v.z);
+    }
+}
+template <class T>
+__device__ __forceinline__ f32x4 round_group(f32x4 v) {   // what a later read of the stored values gives
+    typedef T V __attribute__((ext_vector_type(4)));
+    return __builtin_convertvector(__builtin_convertvector(v, V), f32x4);
+}
+// a parameter vector whose type is only known at run time (its reads are few: once per row at most, from cache)
+__device__ __forceinline__ f32x4 load_param(const void* p, int type, int c, int D) {
+    if (type == T5VQ_F32) return load_group(static_cast<const float*>(p), c, D);
+    if (type == T5VQ_BF16) return load_group(static_cast<const __bf16*>(p), c, D);
+    return load_group(static_cast<const _Float16*>(p), c, D);
+}
+
+// ---- random numbers -------------------------------------------------------------------------------------------------
+// Where a call's random numbers come from (host side): seed / offset by value, or read from device memory on top (a
+// generator under graph capture, or a ticket).
+struct Counter {
+    unsigned long long seed, offset;
+    const long long* seed_dev;
+    const long long* offset_dev;
+    long long* ticket_out;
+};
+struct Drop {               // one dropout site
+    unsigned kept;          // a 16-bit word below this keeps its element; 65536: no dropout, nothing is drawn
+    float scale;            // 65536 / kept: the expectation is the input's, whatever p was rounded to
+};
+inline unsigned kept_of(double p) { return static_cast<unsigned>(t5vq_dropout_keep_count(p)); }
+inline Drop make_drop(double p) {
+    const unsigned k = kept_of(p);
+    return {k, k ? static_cast<float>(65536.0 / k) : 0.f};
+}
+
+struct Key {                // the counter's upper half and the key, the same for a whole site
+    unsigned k0, k1, c0, c1;
+};
+__device__ __forceinline__ Key site_key(const Counter& c, int site) {
+    const unsigned long long seed = c.seed_dev ? static_cast<unsigned long long>(*c.seed_dev) : c.seed;
+    const unsigned long long off =
+        ((c.offset_dev ? static_cast<unsigned long long>(*c.offset_dev) : 0ull) + c.offset) / 4 + site;
+    return {static_cast<unsigned>(seed), static_cast<unsigned>(seed >> 32), static_cast<unsigned>(off),
+            static_cast<unsigned>(off >> 32)};
+}
+__device__ __forceinline__ void give_ticket(const Counter& c) {   // by one thread of the grid: what backward draws from
+    c.ticket_out[0] = c.seed_dev ? *c.seed_dev : static_cast<long long>(c.seed);
+    c.ticket_out[1] = (c.offset_dev ? *c.offset_dev : 0) + static_cast<long long>(c.offset);
+}
+
+struct Words { unsigned w0, w1, w2, w3; };
+// Philox4x32-10 (Salmon, Moraes, Dror, Shaw: "Parallel random numbers: as easy as 1, 2, 3", SC 2011) of the counter
+// (site offset, block of eight columns, row): words 0, 1 belong to the block's lower group of four, 2, 3 to its upper one,
+// 16 bits an element, low half first.  Any lane can draw any element's bits at any time: the mask is never stored.
+__device__ __forceinline__ Words philox(const Key k, unsigned block, unsigned row) {
+    unsigned a = k.c0, b = k.c1, c = block, d = row, k0 = k.k0, k1 = k.k1;
+#pragma unroll
+    for (int i = 0; i < 10; ++i) {
+        const unsigned long long u = static_cast<unsigned long long>(a) * 0xD2511F53u;
+        const unsigned long long v = static_cast<unsigned long long>(c) * 0xCD9E8D57u;
+        a = static_cast<unsigned>(v >> 32) ^ b ^ k0;
+        b = static_cast<unsigned>(v);
+        c = static_cast<unsigned>(u >> 32) ^ d ^ k1;
+        d = static_cast<unsigned>(u);
+        k0 += 0x9E3779B9u;
+        k1 += 0xBB67AE85u;
+    }
+    return {a, b, c, d};
+}
+// A dropped element is 0 whatever it held (an infinity or NaN included).
+__device__ __forceinline__ f32x4 drop_group(f32x4 v, unsigned lo, unsigned hi, Drop d) {
+    v.x = (lo & 0xFFFFu) < d.kept ? v.x * d.scale : 0.f;
+    v.y = (lo >> 16) < d.kept ? v.y * d.scale : 0.f;
+    v.z = (hi & 0xFFFFu) < d.kept ? v.z * d.scale : 0.f;
+    v.w = (hi >> 16) < d.kept ? v.w * d.scale : 0.f;
+    return v;
+}
+__device__ __forceinline__ f32x4 drop_at(f32x4 v, Key k, int q, unsigned row, Drop d) {   // group q of a row, by itself
+    const Words w = philox(k, static_cast<unsigned>(q) >> 1, row);
+    return (q & 1) ? drop_group(v, w.w2, w.w3, d) : drop_group(v, w.w0, w.w1, d);
+}
+
+__device__ __forceinline__ float wave_sum(float v) {   // xor butterfly: the order every row norm of the library uses
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+}
+__device__ __forceinline__ float sq4(const f32x4 v, float s) {
+    s = fmaf(v.x, v.x, s);
+    s = fmaf(v.y, v.y, s);
+    s = fmaf(v.z, v.z, s);
+    s = fmaf(v.w, v.w, s);
+    return s;
+}
+__device__ __forceinline__ float sum4(const f32x4 v, float s) { return s + ((v.x + v.y) + (v.z + v.w)); }
+
+inline bool known_type(int t) { return t == T5VQ_F32 || t == T5VQ_BF16 || t == T5VQ_F16; }
+inline int64_t type_bytes(int t) { return t == T5VQ_F32 ? 4 : 2; }
+inline bool aligned_to(const void* p, int type) {
+    return (reinterpret_cast<uintptr_t>(p) & static_cast<uintptr_t>(type_bytes(type) - 1)) == 0;
+}
+
+}  // namespace t5vq_norm
+#endif

@@ -1,0 +1,246 @@
+// t5vq_norm.hip -- dropout from a counter, and the norms of an encoder with that dropout: forward.  gfx950 kernels + C ABI;
+// include/t5vq.h has the contract.  Backward: t5vq_norm_backward.hip.
+//
+// Compiled with -ffp-contract=off: every fused multiply-add below is an explicit fmaf().
+#include "t5vq_norm.h"
+
+using namespace t5vq_norm;
+
+namespace {
+
+// y = residual + (kept ? x * scale : 0): one thread per block of eight columns, so each Philox block is drawn once.
+template <class TX, class TY, bool RES>
+__global__ __launch_bounds__(256) void dropout_add_kernel(const TX* __restrict__ x, const TY* __restrict__ res, int D,
+                                                          long long blocks, int per_row, Drop drop, Counter ctr,
+                                                          TY* __restrict__ y) {
+    if (ctr.ticket_out && blockIdx.x == 0 && threadIdx.x == 0) give_ticket(ctr);
+    const long long b = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+    if (b >= blocks) return;
+    const long long row = b / per_row;
+    const int blk = static_cast<int>(b - row * per_row), c = blk * 8;
+    const TX* xr = x + row * D;
+    f32x4 lo = load_group(xr, c, D), hi = load_group(xr, c + 4, D);
+    if (drop.kept < 65536u) {
+        const Words w = philox(site_key(ctr, 0), blk, static_cast<unsigned>(row));
+        lo = drop_group(lo, w.w0, w.w1, drop);
+        hi = drop_group(hi, w.w2, w.w3, drop);
+    }
+    if constexpr (RES) {
+        const TY* rr = res + row * D;
+        lo = load_group(rr, c, D) + lo;
+        hi = load_group(rr, c + 4, D) + hi;
+    }
+    store_group(y + row * D, c, D, lo);
+    store_group(y + row * D, c + 4, D, hi);
+}
+
+struct NormArgs {
+    const void* weight;
+    const void* bias;
+    int weight_type, layer, D;
+    long long N;
+    float eps;
+    Drop branch, out;
+    Counter ctr;
+    float* stats;     // [N, 2]: mean (0 for rms), 1 / sqrt(variance + eps)
+    float* xx;        // [N]
+    T5vqTokenImage img;
+};
+
+__device__ __forceinline__ float block_sum(float v, float* slots) {   // 256 threads; fixed order
+    v = wave_sum(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) slots[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return (slots[0] + slots[1]) + (slots[2] + slots[3]);
+}
+
+// One workgroup per row, the row read again from memory for each of its sums: right for every length.
+template <class TH, class TB, class TO, bool ADD>
+__global__ __launch_bounds__(256) void norm_rows_kernel(const TH* __restrict__ hidden, const TB* __restrict__ branch,
+                                                        TO* __restrict__ out, TH* __restrict__ sum, NormArgs a) {
+    __shared__ float slots[4];
+    const int tid = threadIdx.x, D = a.D;
+    if (a.ctr.ticket_out && blockIdx.x == 0 && tid == 0) give_ticket(a.ctr);
+    const bool drops = ADD && a.branch.kept < 65536u;
+    const Key k0 = site_key(a.ctr, 0), k1 = site_key(a.ctr, 1);
+    for (long long row = blockIdx.x; row < a.N; row += gridDim.x) {
+        auto group = [&](int q) {
+            f32x4 h = load_group(hidden + row * D, 4 * q, D);
+            if constexpr (ADD) {
+                f32x4 b = load_group(branch + row * D, 4 * q, D);
+                if (drops) b = drop_at(b, k0, q, static_cast<unsigned>(row), a.branch);
+                h = round_group<TH>(h + b);
+            }
+            return h;
+        };
+        const int groups = (D + 3) / 4;
+        float s = 0.f, mean = 0.f;
+        if (a.layer) {
+            for (int q = tid; q < groups; q += 256) s = sum4(group(q), s);
+            mean = block_sum(s, slots) / static_cast<float>(D);
+        }
+        s = 0.f;
+        for (int q = tid; q < groups; q += 256) {
+            const f32x4 h = group(q);
+            if constexpr (ADD) store_group(sum + row * D, 4 * q, D, h);
+            f32x4 d = h - mean;
+            if (4 * q + 1 >= D) d.y = 0.f;
+            if (4 * q + 2 >= D) d.z = 0.f;
+            if (4 * q + 3 >= D) d.w = 0.f;
+            s = sq4(d, s);
+        }
+        const float r = 1.0f / __fsqrt_rn(block_sum(s, slots) / static_cast<float>(D) + a.eps);
+        if (a.stats && tid == 0) {
+            a.stats[2 * row] = mean;
+            a.stats[2 * row + 1] = r;
+        }
+        for (int q = tid; q < groups; q += 256) {
+            f32x4 y = (group(q) - mean) * r * load_param(a.weight, a.weight_type, 4 * q, D);
+            if (a.bias) y += load_param(a.bias, a.weight_type, 4 * q, D);
+            if (a.out.kept < 65536u) y = drop_at(y, k1, q, static_cast<unsigned>(row), a.out);
+            store_group(out + row * D, 4 * q, D, y);
+        }
+    }
+}
+
+// |row|^2 and the fp16 image of fp32 rows just written: one wave per row, in the library's order of a row norm
+__global__ __launch_bounds__(256) void norm_row_outputs_kernel(const float* __restrict__ out, long long N, int D,
+                                                               float* __restrict__ xx, T5vqTokenImage img) {
+    const int lane = threadIdx.x & 63;
+    const long long row = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    if (row >= N) return;
+    const float* p = out + row * D;
+    float s = 0.f, m = 0.f;
+    for (int c = 4 * lane; c < D; c += 256) {
+        const f32x4 v = load_group(p, c, D);
+        s = sq4(v, s);
+        m = t5vq_absmax4(m, v.x, v.y, v.z, v.w);
+    }
+    s = wave_sum(s);
+    if (xx && lane == 0) xx[row] = s;
+    if (!img.rows) return;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    float inv;
+    const float sc = t5vq_image_scale(m, &inv);
+    if (lane == 0) img.inv[row] = inv;
+    for (int c = 4 * lane; c < D; c += 256) {
+        const f32x4 v = load_group(p, c, D);
+        t5vq_image_store4(img.rows + row * D, c >> 2, v.x, v.y, v.z, v.w, sc);
+    }
+}
+
+template <class TH, class TB, class TO, bool ADD>
+void launch_norm(const void* hidden, const void* branch, void* out, void* sum, int64_t N, const NormArgs& a,
+                 hipStream_t stream) {
+    hipLaunchKernelGGL((norm_rows_kernel<TH, TB, TO, ADD>), dim3(static_cast<unsigned>(N < (1 << 20) ? N : (1 << 20))),
+                       dim3(256), 0, stream, static_cast<const TH*>(hidden), static_cast<const TB*>(branch), static_cast<TO*>(out),
+                       static_cast<TH*>(sum), a);
+}
+
+template <class TX, class TY>
+void launch_dropout(const void* x, const void* res, void* y, int64_t N, int64_t D, Drop drop, const Counter& ctr,
+                    hipStream_t stream) {
+    const int64_t per_row = (D + 7) / 8, blocks = N * per_row;
+    const dim3 grid(static_cast<unsigned>((blocks + 255) / 256));
+    if (res)
+        hipLaunchKernelGGL((dropout_add_kernel<TX, TY, true>), grid, dim3(256), 0, stream, static_cast<const TX*>(x),
+                           static_cast<const TY*>(res), static_cast<int>(D), blocks, static_cast<int>(per_row), drop, ctr,
+                           static_cast<TY*>(y));
+    else
+        hipLaunchKernelGGL((dropout_add_kernel<TX, TY, false>), grid, dim3(256), 0, stream, static_cast<const TX*>(x),
+                           static_cast<const TY*>(res), static_cast<int>(D), blocks, static_cast<int>(per_row), drop, ctr,
+                           static_cast<TY*>(y));
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t t5vq_dropout_keep_count(double p) {
+    if (!(p >= 0.0 && p <= 1.0)) return -1;
+    return static_cast<int64_t>(__builtin_rint((1.0 - p) * 65536.0));   // round half to even
+}
+
+int t5vq_dropout_add(const void* x, int x_type, const void* residual, int64_t N, int64_t D, double p, int64_t seed,
+                     int64_t offset, const int64_t* seed_dev, const int64_t* offset_dev, int64_t* ticket_out, void* y,
+                     int y_type, t5vq_stream_t stream) {
+    T5VQ_I_REQUIRE(x && y, "null pointer");
+    T5VQ_I_REQUIRE(known_type(x_type) && known_type(y_type), "unknown element type");
+    T5VQ_I_REQUIRE(x_type == y_type || x_type == T5VQ_F32 || y_type == T5VQ_F32, "bf16 and f16 do not meet in one call");
+    T5VQ_I_REQUIRE(N > 0 && N <= 0xFFFFFFFFLL && D > 0 && D <= (1LL << 30), "N, D out of range");
+    T5VQ_I_REQUIRE(N * ((D + 7) / 8) <= 0xFFFFFF00LL, "more than 2^35 elements in one launch");
+    T5VQ_I_REQUIRE(t5vq_dropout_keep_count(p) >= 0, "p must be in [0, 1]");
+    T5VQ_I_REQUIRE(aligned_to(x, x_type) && aligned_to(y, y_type) && (!residual || aligned_to(residual, y_type)),
+                   "elements must be aligned");
+    const Drop drop = make_drop(p);
+    const Counter ctr = {static_cast<unsigned long long>(seed), static_cast<unsigned long long>(offset),
+                         reinterpret_cast<const long long*>(seed_dev), reinterpret_cast<const long long*>(offset_dev),
+                         reinterpret_cast<long long*>(ticket_out)};
+    hipStream_t s = static_cast<hipStream_t>(stream);
+#define T5VQ_DA(X, Y) launch_dropout<X, Y>(x, residual, y, N, D, drop, ctr, s)
+    if (x_type == T5VQ_F32 && y_type == T5VQ_F32) T5VQ_DA(float, float);
+    else if (x_type == T5VQ_BF16 && y_type == T5VQ_BF16) T5VQ_DA(__bf16, __bf16);
+    else if (x_type == T5VQ_F16 && y_type == T5VQ_F16) T5VQ_DA(_Float16, _Float16);
+    else if (x_type == T5VQ_BF16) T5VQ_DA(__bf16, float);
+    else if (x_type == T5VQ_F16) T5VQ_DA(_Float16, float);
+    else if (y_type == T5VQ_BF16) T5VQ_DA(float, __bf16);
+    else T5VQ_DA(float, _Float16);
+#undef T5VQ_DA
+    T5VQ_I_CHECK_HIP(hipGetLastError());
+    return T5VQ_OK;
+}
+
+int t5vq_norm_forward(const void* hidden, int hidden_type, const void* branch, int branch_type, const void* weight,
+                      const void* bias, int weight_type, int norm_kind, float eps, int64_t N, int64_t D, double branch_p,
+                      double p, int64_t seed, int64_t offset, const int64_t* seed_dev, const int64_t* offset_dev,
+                      int64_t* ticket_out, void* out, int out_type, void* sum, float* stats, float* xx,
+                      void* token_image, t5vq_stream_t stream) {
+    T5VQ_I_REQUIRE(hidden && weight && out && (!branch || sum), "null pointer");
+    T5VQ_I_REQUIRE(known_type(hidden_type) && known_type(weight_type) && known_type(out_type), "unknown element type");
+    T5VQ_I_REQUIRE(out_type == hidden_type || out_type == T5VQ_F32, "out is of hidden's type or fp32");
+    T5VQ_I_REQUIRE(!branch || branch_type == hidden_type || (hidden_type == T5VQ_F32 && known_type(branch_type)),
+                   "branch is of hidden's type, or hidden is fp32");
+    T5VQ_I_REQUIRE(norm_kind == T5VQ_NORM_LAYER || norm_kind == T5VQ_NORM_RMS, "unknown norm");
+    T5VQ_I_REQUIRE(eps >= 0.f, "eps must not be negative");
+    T5VQ_I_REQUIRE(N > 0 && N <= (1LL << 32) - 1 && D > 0 && D <= (1LL << 30), "N, D out of range");
+    T5VQ_I_REQUIRE(t5vq_dropout_keep_count(p) >= 0 && t5vq_dropout_keep_count(branch_p) >= 0, "p must be in [0, 1]");
+    T5VQ_I_REQUIRE(aligned_to(hidden, hidden_type) && aligned_to(weight, weight_type) && aligned_to(out, out_type) &&
+                       (!bias || aligned_to(bias, weight_type)) &&
+                       (!branch || (aligned_to(branch, branch_type) && aligned_to(sum, hidden_type))),
+                   "elements must be aligned");
+    T5VQ_I_REQUIRE((!xx && !token_image) || (out_type == T5VQ_F32 && D % 4 == 0 && D <= 2048 && N < (1LL << 26)),
+                   "row norms and images are those of fp32 rows, D % 4 == 0, D <= 2048, N < 2^26");
+    T5VQ_I_REQUIRE((reinterpret_cast<uintptr_t>(token_image) & 255u) == 0, "token_image must be 256-byte aligned");
+    NormArgs a;
+    a.weight = weight, a.bias = bias, a.weight_type = weight_type, a.layer = norm_kind == T5VQ_NORM_LAYER;
+    a.D = static_cast<int>(D), a.N = N, a.eps = eps;
+    a.branch = make_drop(branch ? branch_p : 0.0), a.out = make_drop(p);
+    a.ctr = {static_cast<unsigned long long>(seed), static_cast<unsigned long long>(offset),
+             reinterpret_cast<const long long*>(seed_dev), reinterpret_cast<const long long*>(offset_dev),
+             reinterpret_cast<long long*>(ticket_out)};
+    a.stats = stats, a.xx = xx, a.img = t5vq_token_image_parts(token_image, N, D);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+#define T5VQ_NF(H, B, O, ADD) launch_norm<H, B, O, ADD>(hidden, branch, out, sum, N, a, s)
+#define T5VQ_NF_HALF(H)                                                                         \
+    (out_type == T5VQ_F32 ? (branch ? T5VQ_NF(H, H, float, true) : T5VQ_NF(H, H, float, false)) \
+                          : (branch ? T5VQ_NF(H, H, H, true) : T5VQ_NF(H, H, H, false)))
+    if (hidden_type == T5VQ_BF16) T5VQ_NF_HALF(__bf16);
+    else if (hidden_type == T5VQ_F16) T5VQ_NF_HALF(_Float16);
+    else if (!branch) T5VQ_NF(float, float, float, false);
+    else if (branch_type == T5VQ_F32) T5VQ_NF(float, float, float, true);
+    else if (branch_type == T5VQ_BF16) T5VQ_NF(float, __bf16, float, true);
+    else T5VQ_NF(float, _Float16, float, true);
+#undef T5VQ_NF_HALF
+#undef T5VQ_NF
+    T5VQ_I_CHECK_HIP(hipGetLastError());
+    if (xx || token_image) {
+        hipLaunchKernelGGL(norm_row_outputs_kernel, dim3(static_cast<unsigned>((N + 3) / 4)), dim3(256), 0, s,
+                           static_cast<const float*>(out), static_cast<long long>(N), a.D, a.xx, a.img);
+        T5VQ_I_CHECK_HIP(hipGetLastError());
+    }
+    return T5VQ_OK;
+}
+
+}  // extern "C"

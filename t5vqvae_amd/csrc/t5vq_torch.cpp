@@ -9,9 +9,11 @@
 // loaded with torch.ops.load_library (t5vqvae_amd/_lib.py).
 #include <ATen/ATen.h>
 #include <ATen/hip/HIPContext.h>
+#include <ATen/hip/HIPGeneratorImpl.h>
 #include <c10/core/DeviceGuard.h>
 #include <torch/library.h>
 
+#include <mutex>
 #include <optional>
 #include <tuple>
 
@@ -321,6 +323,184 @@ Tensor code_sqnorms(const Tensor& w) {
     return ee;
 }
 
+// ---- dropout from a counter, layer / RMS norm, add + norm (include/t5vq.h) ---------------------------------------------
+int type_of(const Tensor& t, const char* name) {
+    switch (t.scalar_type()) {
+        case at::kFloat: return T5VQ_F32;
+        case at::kBFloat16: return T5VQ_BF16;
+        case at::kHalf: return T5VQ_F16;
+        default: TORCH_CHECK(false, name, " must be float32, bfloat16 or float16, got ", t.scalar_type());
+    }
+}
+int need_rows(const Tensor& t, const char* name, const Tensor& ref) {   // [N, D] rows beside ref's, of any of the three types
+    TORCH_CHECK(t.is_cuda(), name, " must live on a ROCm device (got ", t.device(), "); t5vqvae_amd has no CPU path");
+    TORCH_CHECK(t.dim() == 2 && t.sizes() == ref.sizes(), name, " must be [N, D] like the rows of the call, got ", t.sizes());
+    TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
+    TORCH_CHECK(t.device() == ref.device(), name, " is on ", t.device(), ", expected ", ref.device());
+    return type_of(t, name);
+}
+int need_param(const Tensor& t, const char* name, const Tensor& rows) {
+    TORCH_CHECK(t.is_cuda() && t.device() == rows.device(), name, " is on ", t.device(), ", expected ", rows.device());
+    TORCH_CHECK(t.dim() == 1 && t.size(0) == rows.size(1) && t.is_contiguous(), name, " must be a contiguous vector of ",
+                rows.size(1), " elements, got shape ", t.sizes());
+    return type_of(t, name);
+}
+
+// Where a forward call's random numbers come from: the caller's ticket, or the device's default generator of torch, which
+// is moved on by 8 (two sites of 4) under its lock -- inside a graph capture its state stays on the device and every replay
+// draws anew.
+struct Draw {
+    int64_t seed = 0, offset = 0;
+    const int64_t *seed_dev = nullptr, *offset_dev = nullptr;
+    OptTensor ticket;       // made by this call
+    int64_t* ticket_out = nullptr;
+};
+Draw draw_for(bool drops, const OptTensor& given, const Tensor& rows) {
+    Draw d;
+    if (given.has_value()) {
+        TORCH_CHECK(need(*given, "ticket", at::kLong, 1).numel() == 2, "ticket must hold {seed, offset}");
+        same_device(rows, given, "ticket");
+    }
+    if (!drops) return d;
+    if (given.has_value()) {
+        d.seed_dev = given->data_ptr<int64_t>();
+        d.offset_dev = d.seed_dev + 1;
+        return d;
+    }
+    auto* gen = at::get_generator_or_default<at::CUDAGeneratorImpl>(
+        std::nullopt, at::cuda::detail::getDefaultCUDAGenerator(rows.device().index()));
+    at::PhiloxCudaState st;
+    {
+        const std::lock_guard<std::mutex> lock(gen->mutex_);
+        st = gen->philox_cuda_state(8);
+    }
+    if (st.captured_) {
+        d.seed_dev = reinterpret_cast<const int64_t*>(st.seed_.ptr);
+        d.offset_dev = reinterpret_cast<const int64_t*>(st.offset_.ptr);
+        d.offset = static_cast<int64_t>(st.offset_intragraph_);
+    } else {
+        d.seed = static_cast<int64_t>(st.seed_.val);
+        d.offset = static_cast<int64_t>(st.offset_.val);
+    }
+    d.ticket = at::empty({2}, rows.options().dtype(at::kLong));
+    d.ticket_out = d.ticket->data_ptr<int64_t>();
+    return d;
+}
+bool drops(double p, const char* name) {
+    const int64_t kept = t5vq_dropout_keep_count(p);
+    TORCH_CHECK(kept >= 0, name, " must be in [0, 1], got ", p);
+    return kept < 65536;
+}
+
+// y = residual + dropout(x), of residual's type (x's without one).  Returns (y, the ticket drawn or None).
+std::tuple<Tensor, OptTensor> dropout_add(const Tensor& x, const OptTensor& residual, double p, const OptTensor& ticket) {
+    const c10::DeviceGuard guard(x.device());
+    const int xt = need_rows(x, "x", x);
+    const int yt = residual.has_value() ? need_rows(*residual, "residual", x) : xt;
+    Draw d = draw_for(drops(p, "p"), ticket, x);
+    Tensor y = residual.has_value() ? at::empty_like(*residual) : at::empty_like(x);
+    if (x.numel() == 0) return {y, d.ticket.has_value() ? OptTensor(d.ticket->zero_()) : OptTensor()};
+    ok(t5vq_dropout_add(x.data_ptr(), xt, ptr<void>(residual), x.size(0), x.size(1), p, d.seed, d.offset, d.seed_dev,
+                        d.offset_dev, d.ticket_out, y.data_ptr(), yt, stream_of(x)),
+       "dropout_add");
+    return {y, d.ticket};
+}
+
+// gradient of x from that of y, in x's type (default: g's)
+Tensor dropout_backward(const Tensor& g, double p, const OptTensor& ticket, std::optional<at::ScalarType> dtype) {
+    const c10::DeviceGuard guard(g.device());
+    const int gt = need_rows(g, "g", g);
+    TORCH_CHECK(!drops(p, "p") || ticket.has_value(), "dropout needs the forward's ticket");
+    const Draw d = draw_for(drops(p, "p"), ticket, g);
+    Tensor out = at::empty(g.sizes(), dtype.has_value() ? g.options().dtype(*dtype) : g.options());
+    if (g.numel() == 0) return out;
+    ok(t5vq_dropout_add(g.data_ptr(), gt, nullptr, g.size(0), g.size(1), p, 0, 0, d.seed_dev, d.offset_dev, nullptr,
+                        out.data_ptr(), type_of(out, "dtype"), stream_of(g)),
+       "dropout_backward");
+    return out;
+}
+
+// Returns (out, sum | None, stats | None, row norms | None, ticket drawn | None).
+std::tuple<Tensor, OptTensor, OptTensor, OptTensor, OptTensor> norm_forward(
+    const Tensor& hidden, const OptTensor& branch, const Tensor& weight, const OptTensor& bias, int64_t kind, double eps,
+    double branch_p, double p, const OptTensor& ticket, std::optional<at::ScalarType> out_dtype, bool want_stats,
+    bool want_row_norms, const OptTensor& token_image) {
+    const c10::DeviceGuard guard(hidden.device());
+    const int ht = need_rows(hidden, "hidden", hidden), wt = need_param(weight, "weight", hidden);
+    const int bt = branch.has_value() ? need_rows(*branch, "branch", hidden) : ht;
+    if (bias.has_value())
+        TORCH_CHECK(need_param(*bias, "bias", hidden) == wt, "bias must be of weight's type, ", weight.scalar_type());
+    const int64_t N = hidden.size(0), D = hidden.size(1);
+    if (token_image.has_value()) {
+        TORCH_CHECK(need(*token_image, "token_image", at::kByte).numel() >= t5vq_token_image_bytes(N, D),
+                    "token_image smaller than t5vq_token_image_bytes(N, D)");
+        same_device(hidden, token_image, "token_image");
+    }
+    const bool drops_branch = drops(branch_p, "branch_p") && branch.has_value(), drops_out = drops(p, "p");
+    Draw d = draw_for(drops_branch || drops_out, ticket, hidden);
+    Tensor out = at::empty(hidden.sizes(), out_dtype.has_value() ? hidden.options().dtype(*out_dtype) : hidden.options());
+    const int ot = type_of(out, "out_dtype");
+    const auto f32 = hidden.options().dtype(at::kFloat);
+    OptTensor sum, stats, xx;
+    if (branch.has_value()) sum = at::empty_like(hidden);
+    if (want_stats) stats = at::empty({N, 2}, f32);
+    if (want_row_norms) xx = at::empty({N}, f32);
+    if (hidden.numel() == 0) {
+        if (d.ticket.has_value()) d.ticket->zero_();
+        if (want_stats) stats->zero_();
+        if (want_row_norms) xx->zero_();
+        return {out, sum, stats, xx, d.ticket};
+    }
+    ok(t5vq_norm_forward(hidden.data_ptr(), ht, ptr<void>(branch), bt, weight.data_ptr(), ptr<void>(bias), wt,
+                         static_cast<int>(kind), static_cast<float>(eps), N, D, branch.has_value() ? branch_p : 0.0, p, d.seed,
+                         d.offset, d.seed_dev, d.offset_dev, d.ticket_out, out.data_ptr(), ot, ptr<void>(sum), ptr(stats),
+                         ptr(xx), ptr<void>(token_image), stream_of(hidden)),
+       "norm_forward");
+    return {out, sum, stats, xx, d.ticket};
+}
+
+// Returns (grad_hidden, grad_branch | None, grad_weight | None, grad_bias | None).
+std::tuple<Tensor, OptTensor, OptTensor, OptTensor> norm_backward(
+    const Tensor& g_out, const OptTensor& g_sum, const Tensor& h, const Tensor& weight, const Tensor& stats, int64_t kind,
+    double branch_p, double p, const OptTensor& ticket, std::optional<at::ScalarType> branch_dtype, bool want_weight,
+    bool want_bias) {
+    const c10::DeviceGuard guard(h.device());
+    const int ht = need_rows(h, "h", h), ot = need_rows(g_out, "g_out", h), wt = need_param(weight, "weight", h);
+    if (g_sum.has_value()) TORCH_CHECK(need_rows(*g_sum, "g_sum", h) == ht, "g_sum must be of h's type, ", h.scalar_type());
+    const int64_t N = h.size(0), D = h.size(1);
+    TORCH_CHECK(need(stats, "stats", at::kFloat, 2).size(0) == N && stats.size(1) == 2, "stats must be [", N, ", 2]");
+    TORCH_CHECK(stats.device() == h.device(), "stats is on ", stats.device(), ", expected ", h.device());
+    const bool any = drops(p, "p") || (drops(branch_p, "branch_p") && branch_dtype.has_value());
+    TORCH_CHECK(!any || ticket.has_value(), "dropout needs the forward's ticket");
+    const Draw d = draw_for(any, ticket, h);
+    Tensor gh = at::empty_like(h);
+    OptTensor gb, gw, gbias;
+    int bt = ht;
+    if (branch_dtype.has_value()) {
+        gb = at::empty(h.sizes(), h.options().dtype(*branch_dtype));
+        bt = type_of(*gb, "branch_dtype");
+    }
+    if (want_weight) gw = at::empty_like(weight);
+    if (want_bias) gbias = at::empty_like(weight);
+    if (h.numel() == 0) {
+        if (want_weight) gw->zero_();
+        if (want_bias) gbias->zero_();
+        return {gh, gb, gw, gbias};
+    }
+    Tensor ws;
+    int64_t ws_bytes = 0;
+    if (want_weight || want_bias) {
+        ws_bytes = t5vq_norm_backward_workspace_bytes(N, D);
+        ws = at::empty({ws_bytes}, h.options().dtype(at::kByte));
+    }
+    ok(t5vq_norm_backward(g_out.data_ptr(), ot, ptr<void>(g_sum), h.data_ptr(), ht, weight.data_ptr(), wt,
+                          static_cast<int>(kind), stats.data_ptr<float>(), N, D, branch_p, p, d.seed_dev, gh.data_ptr(),
+                          ptr<void>(gb), bt, ptr<void>(gw), ptr<void>(gbias), ws_bytes ? ws.data_ptr() : nullptr, ws_bytes,
+                          stream_of(h)),
+       "norm_backward");
+    return {gh, gb, gw, gbias};
+}
+
 // Tensors that are not on a ROCm device: there is no CPU path, say so instead of the dispatcher's listing
 void no_cpu_path(const c10::OperatorHandle& op, c10::Stack*) {
     TORCH_CHECK(false, op.schema().name(), ": tensors must live on a ROCm device; t5vqvae_amd has no CPU path");
@@ -350,6 +530,14 @@ TORCH_LIBRARY(t5vq, m) {
     m.def("distances(Tensor x, Tensor w) -> Tensor");
     m.def("one_hot(Tensor idx, int K) -> Tensor");
     m.def("code_sqnorms(Tensor w) -> Tensor");
+    m.def("dropout_add(Tensor x, Tensor? residual, float p, Tensor? ticket=None) -> (Tensor, Tensor?)");
+    m.def("dropout_backward(Tensor g, float p, Tensor? ticket, ScalarType? dtype=None) -> Tensor");
+    m.def("norm_forward(Tensor hidden, Tensor? branch, Tensor weight, Tensor? bias, int kind, float eps, float branch_p, "
+          "float p, Tensor? ticket, ScalarType? out_dtype, bool want_stats, bool want_row_norms=False, "
+          "Tensor(a!)? token_image=None) -> (Tensor, Tensor?, Tensor?, Tensor?, Tensor?)");
+    m.def("norm_backward(Tensor g_out, Tensor? g_sum, Tensor h, Tensor weight, Tensor stats, int kind, float branch_p, "
+          "float p, Tensor? ticket, ScalarType? branch_dtype, bool want_weight, bool want_bias) -> "
+          "(Tensor, Tensor?, Tensor?, Tensor?)");
 }
 
 TORCH_LIBRARY_IMPL(t5vq, CUDA, m) {   // ROCm devices carry the CUDA dispatch key in torch
@@ -362,10 +550,15 @@ TORCH_LIBRARY_IMPL(t5vq, CUDA, m) {   // ROCm devices carry the CUDA dispatch ke
     m.impl("distances", &distances);
     m.impl("one_hot", &one_hot);
     m.impl("code_sqnorms", &code_sqnorms);
+    m.impl("dropout_add", &dropout_add);
+    m.impl("dropout_backward", &dropout_backward);
+    m.impl("norm_forward", &norm_forward);
+    m.impl("norm_backward", &norm_backward);
 }
 
 TORCH_LIBRARY_IMPL(t5vq, CPU, m) {
     for (const char* name : {"vq_forward", "vq_finalize", "vq_step", "ste_backward", "scatter_rows", "cosine_backward",
-                             "distances", "one_hot", "code_sqnorms"})
+                             "distances", "one_hot", "code_sqnorms", "dropout_add", "dropout_backward", "norm_forward",
+                             "norm_backward"})
         m.impl(name, torch::CppFunction::makeFromBoxedFunction<&no_cpu_path>());
 }

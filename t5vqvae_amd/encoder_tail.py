@@ -15,13 +15,18 @@ drop-in (``VectorQuantizerEMA`` alone) does not need it.
 The dropout mask is drawn with torch's generator (``bernoulli_``) and passed to the kernel as a uint8 tensor, or
 given by the caller (``keep_mask=``); torch's own fused dropout draws a different Philox stream, so masks -- not
 results for a given mask -- differ from eager ``nn.Dropout``.
+
+``EncoderTailVQ(dropout="counter")`` stores no mask: the kernel draws it from a counter and the backward draws it again
+(``t5vqvae_amd.norms``).  That form also takes the sublayer in front of the norm (``branch=``: hidden + dropout(branch) in
+the same pass), encoders that end in a LayerNorm (``norm="layer"``), and bf16 / fp16 hidden states; the quantizer always
+receives fp32.
 """
 from __future__ import annotations
 
 import torch
 from torch import nn
 
-from . import ops
+from . import norms, ops
 
 
 class _TailFunction(torch.autograd.Function):
@@ -48,20 +53,43 @@ class EncoderTailVQ(nn.Module):
     """``vq(dropout(T5LayerNorm(hidden_states)), srl)`` with the norm, the dropout and the row norms in one kernel.
 
     ``vq``: a ``t5vqvae_amd`` quantizer module.  ``weight``: the ``final_layer_norm.weight`` Parameter to share (so
-    checkpoints keep their key), or None for a fresh ``ones(hidden_size)`` (modeling_t5.py:197)."""
+    checkpoints keep their key), or None for a fresh ``ones(hidden_size)`` (modeling_t5.py:197).
+
+    ``dropout``: "stored" (a mask of N * D bytes, drawn by torch or given as ``keep_mask``) or "counter" (no mask).  With
+    "counter": ``norm`` may be "layer" -- ``bias`` then is a Parameter to share, None for a fresh one, or False for none --
+    and the call takes ``branch`` (dropped with ``branch_dropout_rate``, default ``dropout_rate``) and ``ticket``."""
 
     # the norm kernel also writes the fp16 image of its output from this many elements on: at C3 (5e7) tail + filtered
     # step 1226 -> 1214 us; at C1 (2.2e6) the extra buffer and output cost more than the preparation pass they save
     token_image_min_elements = 1 << 24
 
-    def __init__(self, vq, hidden_size: int = 768, eps: float = 1e-6, dropout_rate: float = 0.1, weight=None):
+    def __init__(self, vq, hidden_size: int = 768, eps: float = 1e-6, dropout_rate: float = 0.1, weight=None, *,
+                 norm: str = "rms", bias=None, dropout: str = "stored", branch_dropout_rate=None):
         super().__init__()
+        if dropout not in ("stored", "counter"):
+            raise ValueError(f'dropout must be "stored" or "counter", got {dropout!r}')
+        if norm not in ops.NORM_KINDS:
+            raise ValueError(f'norm must be "rms" or "layer", got {norm!r}')
+        if dropout == "stored" and (norm != "rms" or branch_dropout_rate is not None or
+                                    not (bias is None or bias is False)):
+            raise ValueError('norm="layer", bias and branch_dropout_rate need dropout="counter"')
         self.vq = vq
+        self.norm, self.dropout = norm, dropout
+        self.branch_dropout_rate = float(dropout_rate if branch_dropout_rate is None else branch_dropout_rate)
         self.weight = weight if weight is not None else nn.Parameter(torch.ones(hidden_size))
         self.variance_epsilon = eps
         self.dropout_rate = float(dropout_rate)
+        if bias is None:
+            bias = nn.Parameter(torch.zeros(hidden_size)) if norm == "layer" else False
+        self.bias = None if bias is False else bias
 
-    def forward(self, hidden_states, srl=None, keep_mask=None):
+    def forward(self, hidden_states, srl=None, keep_mask=None, branch=None, ticket=None):
+        if self.dropout == "counter":
+            if keep_mask is not None:
+                raise RuntimeError('keep_mask belongs to dropout="stored"; fix a counter\'s mask with ticket=')
+            return self._forward_counter(hidden_states, srl, branch, ticket)
+        if branch is not None or ticket is not None:
+            raise RuntimeError('branch and ticket need dropout="counter"')
         d = hidden_states.shape[-1]
         flat = hidden_states.reshape(-1, d)
         if flat.dtype != torch.float32:
@@ -77,6 +105,16 @@ class EncoderTailVQ(nn.Module):
         x, xx, ximg = _TailFunction.apply(flat, self.weight, keep, scale, float(self.variance_epsilon),
                                           self._wants_image(flat.shape[0], d, srl))
         return self.vq(x.view(hidden_states.shape), srl, _xx=xx, _ximg=ximg if ximg.numel() else None)
+
+    def _forward_counter(self, hidden_states, srl, branch, ticket):
+        rows = norms._rows(hidden_states, "hidden_states")
+        add = None if branch is None else norms._rows(branch, "branch", hidden_states)
+        n, d = rows.shape
+        p, branch_p = (self.dropout_rate, self.branch_dropout_rate) if self.training else (0.0, 0.0)
+        ximg = ops.token_image(n, d, rows.device) if self._wants_image(n, d, srl) else None
+        x, _, xx = norms._norm_call(rows, add, self.weight, self.bias, self.norm, float(self.variance_epsilon), branch_p, p,
+                                    ticket, torch.float32, row_norms=True, token_image=ximg)
+        return self.vq(x.view(hidden_states.shape), srl, _xx=xx, _ximg=ximg)
 
     def _wants_image(self, n: int, d: int, srl) -> bool:
         """Whether the quantizer's search of this call will be the filtered one in token order -- then the norm kernel

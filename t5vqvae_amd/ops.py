@@ -627,3 +627,51 @@ def cosine_backward(x, q, g_out, g_loss, coef_x: float, coef_q: float, want_grad
 
 def one_hot(idx, k: int):
     return _lib.load_torch_ops().one_hot(idx.reshape(-1), k)
+
+
+# ---- dropout from a counter, layer / RMS norm, add + norm (t5vqvae_amd.norms calls these) --------------------------
+NORM_KINDS = {"layer": 0, "rms": 1}
+
+
+def _norm_kind(kind: str) -> int:
+    if kind not in NORM_KINDS:
+        raise RuntimeError(f"kind must be one of {sorted(NORM_KINDS)}, got {kind!r}")
+    return NORM_KINDS[kind]
+
+
+def dropout_keep_count(p: float) -> int:
+    """Of 65536 equally likely 16-bit draws, how many keep an element (t5vq_dropout_keep_count)."""
+    k = int(_lib.load().t5vq_dropout_keep_count(p))
+    if k < 0:
+        raise RuntimeError(f"p must be in [0, 1], got {p}")
+    return k
+
+
+def dropout_add(x, p: float, residual=None, ticket=None):
+    """(residual + dropout(x), ticket drawn | None): t5vq::dropout_add on [N, D] rows.  ``ticket`` (int64 [2], {seed,
+    offset}) fixes the mask; without one the numbers come from torch's generator of the device."""
+    return _lib.load_torch_ops().dropout_add(x, residual, p, ticket)
+
+
+def dropout_backward(g, p: float, ticket, dtype=None):
+    """Gradient of x of ``dropout_add`` from that of its result, in ``dtype`` (default: g's)."""
+    return _lib.load_torch_ops().dropout_backward(g, p, ticket, dtype)
+
+
+def norm_forward(hidden, weight, bias=None, *, kind: str = "layer", eps: float = 1e-6, branch=None, branch_p: float = 0.0,
+                 p: float = 0.0, ticket=None, out_dtype=None, want_stats: bool = True, want_row_norms: bool = False,
+                 token_image=None):
+    """(out, sum | None, stats | None, xx | None, ticket drawn | None): t5vq::norm_forward on [N, D] rows --
+    sum = hidden + dropout(branch; branch_p), out = dropout(norm(sum or hidden) * weight + bias; p).  ``want_row_norms`` /
+    ``token_image`` (fp32 out, D % 4 == 0, D <= 2048): |out|^2 and the fp16 image of out, as the searches take them."""
+    return _lib.load_torch_ops().norm_forward(hidden, branch, weight, bias, _norm_kind(kind), eps, branch_p, p, ticket,
+                                              out_dtype, want_stats, want_row_norms, token_image)
+
+
+def norm_backward(g_out, g_sum, h, weight, stats, *, kind: str = "layer", branch_p: float = 0.0, p: float = 0.0, ticket=None,
+                  branch_dtype=None, want_weight: bool = True, want_bias: bool = True):
+    """(grad_hidden, grad_branch | None, grad_weight | None, grad_bias | None): t5vq::norm_backward.  ``h``: the rows that
+    were normed (the forward's sum, or hidden); ``g_sum``: gradient into the sum from elsewhere, or None;
+    ``branch_dtype``: also write the branch's gradient, in this type."""
+    return _lib.load_torch_ops().norm_backward(g_out, g_sum, h, weight, stats, _norm_kind(kind), branch_p, p, ticket,
+                                               branch_dtype, want_weight, want_bias)
