@@ -136,6 +136,50 @@ __device__ __forceinline__ float sq4(const f32x4 v, float s) {
 }
 __device__ __forceinline__ float sum4(const f32x4 v, float s) { return s + ((v.x + v.y) + (v.z + v.w)); }
 
+// The dropout of a row held in registers, group lane + G * j in v[j] (G >= 2 lanes a row, G even).  Neighbouring lanes hold
+// the two halves of a block; for two chunks j, j + 1 the even lane draws chunk j's block and the odd lane chunk j + 1's, and
+// each hands its neighbour the two words it needs: half the draws of every lane drawing for itself.
+template <int G, int NCH>
+__device__ __forceinline__ void drop_row(f32x4 (&v)[NCH], Key k, unsigned row, int lane, Drop d) {
+    const bool odd = lane & 1;
+#pragma unroll
+    for (int j = 0; j + 1 < NCH; j += 2) {
+        const Words w = philox(k, static_cast<unsigned>(lane + G * (odd ? j + 1 : j)) >> 1, row);
+        const unsigned s0 = odd ? w.w0 : w.w2, s1 = odd ? w.w1 : w.w3;      // the neighbour's half of my block
+        const unsigned m0 = odd ? w.w2 : w.w0, m1 = odd ? w.w3 : w.w1;      // mine
+        const unsigned r0 = __builtin_amdgcn_mov_dpp(s0, 0xB1, 0xF, 0xF, true);   // quad_perm [1, 0, 3, 2]
+        const unsigned r1 = __builtin_amdgcn_mov_dpp(s1, 0xB1, 0xF, 0xF, true);
+        v[j] = drop_group(v[j], odd ? r0 : m0, odd ? r1 : m1, d);
+        v[j + 1] = drop_group(v[j + 1], odd ? m0 : r0, odd ? m1 : r1, d);
+    }
+    if constexpr (NCH & 1) v[NCH - 1] = drop_at(v[NCH - 1], k, lane + G * (NCH - 1), row, d);
+}
+
+// sum over the G lanes of a row (G: a multiple of 64), fixed order; slots: G / 64 floats of LDS, and one more set for the
+// next call, which may then write before every wave has read this one's
+template <int G>
+__device__ __forceinline__ float row_sum(float v, float* slots) {
+    v = wave_sum(v);
+    if constexpr (G > 64) {
+        if ((threadIdx.x & 63) == 0) slots[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = 0.f;
+#pragma unroll
+        for (int i = 0; i < G / 64; ++i) v += slots[i];
+    }
+    return v;
+}
+// values of columns >= D to 0 (they only exist in a row's last group and behind it)
+__device__ __forceinline__ f32x4 inside(f32x4 v, int c, int D) {
+    if (c + 4 > D) {
+        if (c >= D) v.x = 0.f;
+        if (c + 1 >= D) v.y = 0.f;
+        if (c + 2 >= D) v.z = 0.f;
+        v.w = 0.f;
+    }
+    return v;
+}
+
 inline bool known_type(int t) { return t == T5VQ_F32 || t == T5VQ_BF16 || t == T5VQ_F16; }
 inline int64_t type_bytes(int t) { return t == T5VQ_F32 ? 4 : 2; }
 inline bool aligned_to(const void* p, int type) {

@@ -2,6 +2,8 @@
 // include/t5vq.h has the contract.  Backward: t5vq_norm_backward.hip.
 //
 // Compiled with -ffp-contract=off: every fused multiply-add below is an explicit fmaf().
+#include <type_traits>
+
 #include "t5vq_norm.h"
 
 using namespace t5vq_norm;
@@ -47,6 +49,93 @@ struct NormArgs {
     T5vqTokenImage img;
 };
 
+// A row in registers: G lanes hold it, group lane + G * j in chunk j of NCH.  One read of each input, one write of each
+// output; G = 64 (one wave a row, no barrier) up to 2048 columns, a workgroup a row above.  The parameters stay in registers
+// while a wave walks its rows.
+template <class TH, class TB, class TO, bool ADD, int G, int NCH>
+__global__ __launch_bounds__(G > 256 ? G : 256) void norm_kernel(const TH* __restrict__ hidden, const TB* __restrict__ branch,
+                                                                 TO* __restrict__ out, TH* __restrict__ sum, NormArgs a) {
+    constexpr int WG = G > 256 ? G : 256, ROWS = WG / G;
+    __shared__ float slots[2][G > 64 ? G / 64 : 1];
+    const int lane = threadIdx.x & (G - 1), D = a.D;
+    if (a.ctr.ticket_out && blockIdx.x == 0 && threadIdx.x == 0) give_ticket(a.ctr);
+    const Key k0 = site_key(a.ctr, 0), k1 = site_key(a.ctr, 1);
+    const f32x4 zero4 = {0.f, 0.f, 0.f, 0.f};
+    f32x4 w[NCH], b[NCH];
+#pragma unroll
+    for (int j = 0; j < NCH; ++j) {
+        w[j] = load_param(a.weight, a.weight_type, 4 * (lane + G * j), D);
+        b[j] = a.bias ? load_param(a.bias, a.weight_type, 4 * (lane + G * j), D) : zero4;
+    }
+    const float inv_d = 1.0f / static_cast<float>(D);
+    for (long long row = static_cast<long long>(blockIdx.x) * ROWS + threadIdx.x / G; row < a.N;
+         row += static_cast<long long>(gridDim.x) * ROWS) {
+        f32x4 h[NCH];
+#pragma unroll
+        for (int j = 0; j < NCH; ++j) h[j] = load_group(hidden + row * D, 4 * (lane + G * j), D);
+        if constexpr (ADD) {
+            f32x4 br[NCH];
+#pragma unroll
+            for (int j = 0; j < NCH; ++j) br[j] = load_group(branch + row * D, 4 * (lane + G * j), D);
+            if (a.branch.kept < 65536u) drop_row<G>(br, k0, static_cast<unsigned>(row), lane, a.branch);
+#pragma unroll
+            for (int j = 0; j < NCH; ++j) {
+                h[j] = round_group<TH>(h[j] + br[j]);
+                store_group(sum + row * D, 4 * (lane + G * j), D, h[j]);
+            }
+        }
+        float mean = 0.f, s = 0.f;
+        if (a.layer) {
+#pragma unroll
+            for (int j = 0; j < NCH; ++j) s = sum4(h[j], s);
+            mean = row_sum<G>(s, slots[0]) * inv_d;
+            s = 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < NCH; ++j) {
+            h[j] = inside(h[j] - mean, 4 * (lane + G * j), D);
+            s = sq4(h[j], s);
+        }
+        const float r = 1.0f / __fsqrt_rn(row_sum<G>(s, slots[1]) * inv_d + a.eps);
+        if (a.stats && lane == 0) {
+            a.stats[2 * row] = mean;
+            a.stats[2 * row + 1] = r;
+        }
+#pragma unroll
+        for (int j = 0; j < NCH; ++j) h[j] = h[j] * r * w[j] + b[j];
+        if (a.out.kept < 65536u) drop_row<G>(h, k1, static_cast<unsigned>(row), lane, a.out);
+        float m = 0.f;
+        s = 0.f;
+#pragma unroll
+        for (int j = 0; j < NCH; ++j) {
+            store_group(out + row * D, 4 * (lane + G * j), D, h[j]);
+            if (std::is_same<TO, float>::value && G == 64) {
+                s = sq4(h[j], s);
+                m = t5vq_absmax4(m, h[j].x, h[j].y, h[j].z, h[j].w);
+            }
+        }
+        if constexpr (std::is_same<TO, float>::value && G == 64) {   // what the searches take of fp32 rows (D <= 2048)
+            if (a.xx) {
+                s = wave_sum(s);
+                if (lane == 0) a.xx[row] = s;
+            }
+            if (a.img.rows) {
+#pragma unroll
+                for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+                float inv;
+                const float sc = t5vq_image_scale(m, &inv);
+                if (lane == 0) a.img.inv[row] = inv;
+#pragma unroll
+                for (int j = 0; j < NCH; ++j) {
+                    const int q = lane + G * j;
+                    if (4 * q < D) t5vq_image_store4(a.img.rows + row * D, q, h[j].x, h[j].y, h[j].z, h[j].w, sc);
+                }
+            }
+        }
+        if constexpr (G > 64) __syncthreads();   // the next row's sums reuse the slots
+    }
+}
+
 __device__ __forceinline__ float block_sum(float v, float* slots) {   // 256 threads; fixed order
     v = wave_sum(v);
     __syncthreads();
@@ -55,7 +144,7 @@ __device__ __forceinline__ float block_sum(float v, float* slots) {   // 256 thr
     return (slots[0] + slots[1]) + (slots[2] + slots[3]);
 }
 
-// One workgroup per row, the row read again from memory for each of its sums: right for every length.
+// Rows that registers do not hold (D > 16384): one workgroup per row, read again from memory for each of its sums.
 template <class TH, class TB, class TO, bool ADD>
 __global__ __launch_bounds__(256) void norm_rows_kernel(const TH* __restrict__ hidden, const TB* __restrict__ branch,
                                                         TO* __restrict__ out, TH* __restrict__ sum, NormArgs a) {
@@ -104,39 +193,33 @@ __global__ __launch_bounds__(256) void norm_rows_kernel(const TH* __restrict__ h
     }
 }
 
-// |row|^2 and the fp16 image of fp32 rows just written: one wave per row, in the library's order of a row norm
-__global__ __launch_bounds__(256) void norm_row_outputs_kernel(const float* __restrict__ out, long long N, int D,
-                                                               float* __restrict__ xx, T5vqTokenImage img) {
-    const int lane = threadIdx.x & 63;
-    const long long row = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    if (row >= N) return;
-    const float* p = out + row * D;
-    float s = 0.f, m = 0.f;
-    for (int c = 4 * lane; c < D; c += 256) {
-        const f32x4 v = load_group(p, c, D);
-        s = sq4(v, s);
-        m = t5vq_absmax4(m, v.x, v.y, v.z, v.w);
-    }
-    s = wave_sum(s);
-    if (xx && lane == 0) xx[row] = s;
-    if (!img.rows) return;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-    float inv;
-    const float sc = t5vq_image_scale(m, &inv);
-    if (lane == 0) img.inv[row] = inv;
-    for (int c = 4 * lane; c < D; c += 256) {
-        const f32x4 v = load_group(p, c, D);
-        t5vq_image_store4(img.rows + row * D, c >> 2, v.x, v.y, v.z, v.w, sc);
-    }
-}
+constexpr int64_t MOST_WGS = 2048;   // 256 CUs x 8 workgroups of four waves: what is resident at 64 registers
 
 template <class TH, class TB, class TO, bool ADD>
 void launch_norm(const void* hidden, const void* branch, void* out, void* sum, int64_t N, const NormArgs& a,
                  hipStream_t stream) {
-    hipLaunchKernelGGL((norm_rows_kernel<TH, TB, TO, ADD>), dim3(static_cast<unsigned>(N < (1 << 20) ? N : (1 << 20))),
-                       dim3(256), 0, stream, static_cast<const TH*>(hidden), static_cast<const TB*>(branch), static_cast<TO*>(out),
-                       static_cast<TH*>(sum), a);
+#define T5VQ_NK(G, NCH)                                                                                                     \
+    do {                                                                                                                    \
+        constexpr int64_t rows = G >= 256 ? 1 : 256 / G;                                                                    \
+        const int64_t wgs = (N + rows - 1) / rows;                                                                          \
+        hipLaunchKernelGGL((norm_kernel<TH, TB, TO, ADD, G, NCH>),                                                          \
+                           dim3(static_cast<unsigned>(wgs < MOST_WGS ? wgs : MOST_WGS)), dim3(G > 256 ? G : 256), 0, stream, \
+                           static_cast<const TH*>(hidden), static_cast<const TB*>(branch), static_cast<TO*>(out),           \
+                           static_cast<TH*>(sum), a);                                                                       \
+    } while (0)
+    if (a.D <= 256) T5VQ_NK(64, 1);
+    else if (a.D <= 512) T5VQ_NK(64, 2);
+    else if (a.D <= 768) T5VQ_NK(64, 3);
+    else if (a.D <= 1024) T5VQ_NK(64, 4);
+    else if (a.D <= 2048) T5VQ_NK(64, 8);
+    else if (a.D <= 4096) T5VQ_NK(256, 4);
+    else if (a.D <= 8192) T5VQ_NK(1024, 2);
+    else if (a.D <= 16384) T5VQ_NK(1024, 4);
+    else
+        hipLaunchKernelGGL((norm_rows_kernel<TH, TB, TO, ADD>), dim3(static_cast<unsigned>(N < MOST_WGS ? N : MOST_WGS)),
+                           dim3(256), 0, stream, static_cast<const TH*>(hidden), static_cast<const TB*>(branch),
+                           static_cast<TO*>(out), static_cast<TH*>(sum), a);
+#undef T5VQ_NK
 }
 
 template <class TX, class TY>
@@ -210,8 +293,8 @@ int t5vq_norm_forward(const void* hidden, int hidden_type, const void* branch, i
                        (!bias || aligned_to(bias, weight_type)) &&
                        (!branch || (aligned_to(branch, branch_type) && aligned_to(sum, hidden_type))),
                    "elements must be aligned");
-    T5VQ_I_REQUIRE((!xx && !token_image) || (out_type == T5VQ_F32 && D % 4 == 0 && D <= 2048 && N < (1LL << 26)),
-                   "row norms and images are those of fp32 rows, D % 4 == 0, D <= 2048, N < 2^26");
+    T5VQ_I_REQUIRE((!xx && !token_image) || (out_type == T5VQ_F32 && D % 4 == 0 && D <= 2048),
+                   "row norms and images are those of fp32 rows, D % 4 == 0, D <= 2048");
     T5VQ_I_REQUIRE((reinterpret_cast<uintptr_t>(token_image) & 255u) == 0, "token_image must be 256-byte aligned");
     NormArgs a;
     a.weight = weight, a.bias = bias, a.weight_type = weight_type, a.layer = norm_kind == T5VQ_NORM_LAYER;
@@ -235,11 +318,6 @@ int t5vq_norm_forward(const void* hidden, int hidden_type, const void* branch, i
 #undef T5VQ_NF_HALF
 #undef T5VQ_NF
     T5VQ_I_CHECK_HIP(hipGetLastError());
-    if (xx || token_image) {
-        hipLaunchKernelGGL(norm_row_outputs_kernel, dim3(static_cast<unsigned>((N + 3) / 4)), dim3(256), 0, s,
-                           static_cast<const float*>(out), static_cast<long long>(N), a.D, a.xx, a.img);
-        T5VQ_I_CHECK_HIP(hipGetLastError());
-    }
     return T5VQ_OK;
 }
 
