@@ -25,8 +25,92 @@ __device__ __forceinline__ float block_sum(float v, float* slots) {   // 256 thr
 }
 
 // With gy = kept ? g * scale : 0, a = gy * weight, n = (h - mean) r:
-//   grad_h = r (a - mean(a) - n mean(a n)) (+ g_sum), without mean(a) for rms;  grad_branch = kept ? grad_h * scale : 0.
-// One workgroup per row, the row read once for its two sums and once for the gradients.
+//   grad_h = r (a - mean(a) - n mean(a n)) (+ g_sum), without mean(a) for rms;  grad_branch = kept ? grad_h * scale : 0;
+//   grad_weight = sum over rows of gy n, grad_bias = sum of gy.
+// The row stays in registers between its two sums and its gradients (group lane + G * j in chunk j, as forward), and a wave
+// adds up the parameters' gradients of all rows it walks: every input is read once.  Workgroup b leaves its sums in part[b].
+template <class TO, class TH, class TB, int G, int NCH>
+__global__ __launch_bounds__(G > 256 ? G : 256) void norm_backward_kernel(const TO* __restrict__ g,
+                                                                          const TH* __restrict__ g_sum,
+                                                                          const TH* __restrict__ h, BackArgs a,
+                                                                          TH* __restrict__ grad_h,
+                                                                          TB* __restrict__ grad_branch,
+                                                                          float* __restrict__ part) {
+    constexpr int WG = G > 256 ? G : 256, ROWS = WG / G;
+    __shared__ float slots[2][G > 64 ? G / 64 : 1];
+    __shared__ f32x4 sums[ROWS > 1 ? ROWS : 1][ROWS > 1 ? G * NCH : 1];
+    const int lane = threadIdx.x & (G - 1), D = a.D;
+    const Key k0 = site_key(a.ctr, 0), k1 = site_key(a.ctr, 1);
+    const f32x4 zero4 = {0.f, 0.f, 0.f, 0.f};
+    f32x4 w[NCH], gw[NCH], gb[NCH];
+#pragma unroll
+    for (int j = 0; j < NCH; ++j) {
+        w[j] = load_param(a.weight, a.weight_type, 4 * (lane + G * j), D);
+        gw[j] = zero4;
+        gb[j] = zero4;
+    }
+    const float inv_d = 1.0f / static_cast<float>(D);
+    for (long long row = static_cast<long long>(blockIdx.x) * ROWS + threadIdx.x / G; row < a.N;
+         row += static_cast<long long>(gridDim.x) * ROWS) {
+        f32x4 v[NCH], n[NCH], gs[NCH];
+#pragma unroll
+        for (int j = 0; j < NCH; ++j) {
+            v[j] = load_group(g + row * D, 4 * (lane + G * j), D);
+            n[j] = load_group(h + row * D, 4 * (lane + G * j), D);
+            gs[j] = g_sum ? load_group(g_sum + row * D, 4 * (lane + G * j), D) : zero4;
+        }
+        const float mean = a.stats[2 * row], r = a.stats[2 * row + 1];
+        if (a.out.kept < 65536u) drop_row<G>(v, k1, static_cast<unsigned>(row), lane, a.out);
+        float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int j = 0; j < NCH; ++j) {
+            n[j] = (n[j] - mean) * r;      // behind the row's end g is 0: what n is there reaches no sum
+            gw[j] += v[j] * n[j];
+            gb[j] += v[j];
+            v[j] *= w[j];
+            s1 = sum4(v[j], s1);
+            s2 = sum4(v[j] * n[j], s2);
+        }
+        s1 = a.layer ? row_sum<G>(s1, slots[0]) * inv_d : 0.f;
+        s2 = row_sum<G>(s2, slots[1]) * inv_d;
+#pragma unroll
+        for (int j = 0; j < NCH; ++j) {
+            v[j] = (v[j] - s1 - n[j] * s2) * r + gs[j];
+            store_group(grad_h + row * D, 4 * (lane + G * j), D, v[j]);
+        }
+        if (grad_branch) {
+            if (a.branch.kept < 65536u) drop_row<G>(v, k0, static_cast<unsigned>(row), lane, a.branch);
+#pragma unroll
+            for (int j = 0; j < NCH; ++j) store_group(grad_branch + row * D, 4 * (lane + G * j), D, v[j]);
+        }
+        if constexpr (G > 64) __syncthreads();   // the next row's sums reuse the slots
+    }
+    if (!part) return;
+    float* p = part + static_cast<size_t>(blockIdx.x) * 2 * D;
+    if constexpr (ROWS > 1) {   // the waves' sums, in fixed order
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+#pragma unroll
+            for (int j = 0; j < NCH; ++j) sums[threadIdx.x / G][lane + G * j] = half ? gb[j] : gw[j];
+            __syncthreads();
+            for (int q = threadIdx.x; 4 * q < D; q += WG) {
+                f32x4 t = sums[0][q];
+#pragma unroll
+                for (int i = 1; i < ROWS; ++i) t += sums[i][q];
+                store_group(p + half * D, 4 * q, D, t);
+            }
+            __syncthreads();
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < NCH; ++j) {
+            store_group(p, 4 * (lane + G * j), D, gw[j]);
+            store_group(p + D, 4 * (lane + G * j), D, gb[j]);
+        }
+    }
+}
+
+// Rows that registers do not hold (D > 8192): one workgroup per row, read once for its sums and once for its gradients.
 template <class TO, class TH, class TB>
 __global__ __launch_bounds__(256) void norm_backward_rows_kernel(const TO* __restrict__ g, const TH* __restrict__ g_sum,
                                                                  const TH* __restrict__ h, BackArgs a,
@@ -62,8 +146,7 @@ __global__ __launch_bounds__(256) void norm_backward_rows_kernel(const TO* __res
     }
 }
 
-// Parameter gradients: grad_weight = sum over rows of gy n, grad_bias = sum of gy.  Slice s of the rows leaves its sums in
-// part[s]; norm_param_reduce_kernel adds the slices in fixed order.
+// Their parameters' gradients: slice s of the rows leaves its sums in part[s].
 template <class TO, class TH>
 __global__ __launch_bounds__(256) void norm_param_grad_kernel(const TO* __restrict__ g, const TH* __restrict__ h,
                                                               BackArgs a, float* __restrict__ part) {
@@ -82,40 +165,71 @@ __global__ __launch_bounds__(256) void norm_param_grad_kernel(const TO* __restri
     store_group(p + D, 4 * q, D, gb);
 }
 
-__global__ __launch_bounds__(256) void norm_param_reduce_kernel(const float* __restrict__ part, int slices, int D,
-                                                                void* __restrict__ grad_weight,
-                                                                void* __restrict__ grad_bias, int type) {
-    const int col = blockIdx.x * 256 + threadIdx.x;
+// part[slices][2][D] to the two gradients: 16 columns x 64 slice groups a workgroup, one tree over the groups -- a fixed order
+__global__ __launch_bounds__(1024) void norm_param_reduce_kernel(const float* __restrict__ part, int slices, int D,
+                                                                 void* __restrict__ grad_weight,
+                                                                 void* __restrict__ grad_bias, int type) {
+    __shared__ float sums[64][17];
+    const int c = threadIdx.x & 15, s0 = threadIdx.x >> 4, col = blockIdx.x * 16 + c;
     void* to = blockIdx.y ? grad_bias : grad_weight;
-    if (col >= D || !to) return;
+    if (!to) return;
     const float* p = part + static_cast<size_t>(blockIdx.y) * D + col;
     float acc = 0.f;
-    for (int s = 0; s < slices; ++s) acc += p[static_cast<size_t>(s) * 2 * D];
+    if (col < D)
+        for (int s = s0; s < slices; s += 64) acc += p[static_cast<size_t>(s) * 2 * D];
+    sums[s0][c] = acc;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        __syncthreads();
+        if (s0 < o) sums[s0][c] += sums[s0 + o][c];
+    }
+    if (s0 || col >= D) return;
+    acc = sums[0][c];
     if (type == T5VQ_F32) static_cast<float*>(to)[col] = acc;
     else if (type == T5VQ_BF16) static_cast<__bf16*>(to)[col] = static_cast<__bf16>(acc);
     else static_cast<_Float16*>(to)[col] = static_cast<_Float16>(acc);
 }
 
+// How many workgroups share the rows; each leaves 2 D floats of sums.
+int slices_of(int64_t N, int64_t D) {
+    const int64_t rows = D <= 1024 ? 4 : 1, wgs = (N + rows - 1) / rows, most = D <= 1024 ? 768 : 512;
+    return static_cast<int>(wgs < most ? wgs : most);
+}
+
 template <class TO, class TH, class TB>
 void launch_back(const void* g, const void* g_sum, const void* h, const BackArgs& a, void* grad_h, void* grad_branch,
                  bool params, float* part, int slices, hipStream_t s) {
-    hipLaunchKernelGGL((norm_backward_rows_kernel<TO, TH, TB>),
-                       dim3(static_cast<unsigned>(a.N < (1 << 20) ? a.N : (1 << 20))), dim3(256), 0, s,
-                       static_cast<const TO*>(g), static_cast<const TH*>(g_sum), static_cast<const TH*>(h), a,
-                       static_cast<TH*>(grad_h), static_cast<TB*>(grad_branch));
-    if (params)
-        hipLaunchKernelGGL((norm_param_grad_kernel<TO, TH>), dim3((a.D + 1023) / 1024, slices), dim3(256), 0, s,
-                           static_cast<const TO*>(g), static_cast<const TH*>(h), a, part);
+    const TO* gp = static_cast<const TO*>(g);
+    const TH *gsp = static_cast<const TH*>(g_sum), *hp = static_cast<const TH*>(h);
+    TH* ghp = static_cast<TH*>(grad_h);
+    TB* gbp = static_cast<TB*>(grad_branch);
+    const dim3 grid(slices);
+#define T5VQ_NBK(G, NCH)                                                                                                  \
+    hipLaunchKernelGGL((norm_backward_kernel<TO, TH, TB, G, NCH>), grid, dim3(G > 256 ? G : 256), 0, s, gp, gsp, hp, a,   \
+                       ghp, gbp, params ? part : nullptr)
+    if (a.D <= 256) T5VQ_NBK(64, 1);
+    else if (a.D <= 512) T5VQ_NBK(64, 2);
+    else if (a.D <= 768) T5VQ_NBK(64, 3);
+    else if (a.D <= 1024) T5VQ_NBK(64, 4);
+    else if (a.D <= 2048) T5VQ_NBK(256, 2);
+    else if (a.D <= 4096) T5VQ_NBK(256, 4);
+    else if (a.D <= 8192) T5VQ_NBK(1024, 2);
+    else {
+        hipLaunchKernelGGL((norm_backward_rows_kernel<TO, TH, TB>), dim3(static_cast<unsigned>(a.N < 2048 ? a.N : 2048)),
+                           dim3(256), 0, s, gp, gsp, hp, a, ghp, gbp);
+        if (params)
+            hipLaunchKernelGGL((norm_param_grad_kernel<TO, TH>), dim3((a.D + 1023) / 1024, slices), dim3(256), 0, s, gp, hp, a,
+                               part);
+    }
+#undef T5VQ_NBK
 }
-
-int slices_of(int64_t N) { return static_cast<int>(N < 512 ? N : 512); }
 
 }  // namespace
 
 extern "C" {
 
 int64_t t5vq_norm_backward_workspace_bytes(int64_t N, int64_t D) {
-    return N > 0 && D > 0 ? static_cast<int64_t>(slices_of(N)) * 2 * D * 4 : 0;
+    return N > 0 && D > 0 ? static_cast<int64_t>(slices_of(N, D)) * 2 * D * 4 : 0;
 }
 
 int t5vq_norm_backward(const void* grad_out, int out_type, const void* grad_sum, const void* h, int hidden_type,
@@ -151,7 +265,7 @@ int t5vq_norm_backward(const void* grad_out, int out_type, const void* grad_sum,
              nullptr};
     a.stats = stats;
     float* part = static_cast<float*>(workspace);
-    const int slices = slices_of(N);
+    const int slices = slices_of(N, D);
     hipStream_t s = static_cast<hipStream_t>(stream);
 #define T5VQ_NB(O, H, B) launch_back<O, H, B>(grad_out, grad_sum, h, a, grad_hidden, grad_branch, params, part, slices, s)
     if (hidden_type == T5VQ_BF16) out_type == T5VQ_F32 ? T5VQ_NB(float, __bf16, __bf16) : T5VQ_NB(__bf16, __bf16, __bf16);
@@ -163,7 +277,7 @@ int t5vq_norm_backward(const void* grad_out, int out_type, const void* grad_sum,
 #undef T5VQ_NB
     T5VQ_I_CHECK_HIP(hipGetLastError());
     if (params) {
-        hipLaunchKernelGGL(norm_param_reduce_kernel, dim3(static_cast<unsigned>((D + 255) / 256), 2), dim3(256), 0, s, part,
+        hipLaunchKernelGGL(norm_param_reduce_kernel, dim3(static_cast<unsigned>((D + 15) / 16), 2), dim3(1024), 0, s, part,
                            slices, a.D, grad_weight, grad_bias, weight_type);
         T5VQ_I_CHECK_HIP(hipGetLastError());
     }
