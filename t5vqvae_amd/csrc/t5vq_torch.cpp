@@ -11,6 +11,8 @@
 #include <ATen/hip/HIPContext.h>
 #include <ATen/hip/HIPGeneratorImpl.h>
 #include <c10/core/DeviceGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
 
 #include <mutex>
@@ -332,17 +334,19 @@ int type_of(const Tensor& t, const char* name) {
         default: TORCH_CHECK(false, name, " must be float32, bfloat16 or float16, got ", t.scalar_type());
     }
 }
-int need_rows(const Tensor& t, const char* name, const Tensor& ref) {   // [N, D] rows beside ref's, of any of the three types
+int need_rows(const Tensor& t, const char* name, const Tensor& ref) {   // rows [..., D] beside ref's, of any of the three types
     TORCH_CHECK(t.is_cuda(), name, " must live on a ROCm device (got ", t.device(), "); t5vqvae_amd has no CPU path");
-    TORCH_CHECK(t.dim() == 2 && t.sizes() == ref.sizes(), name, " must be [N, D] like the rows of the call, got ", t.sizes());
+    TORCH_CHECK(t.dim() >= 1 && t.size(-1) > 0, name, " must be rows [..., D] with D > 0, got shape ", t.sizes());
+    TORCH_CHECK(t.sizes() == ref.sizes(), name, " must have shape ", ref.sizes(), ", got ", t.sizes());
     TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
     TORCH_CHECK(t.device() == ref.device(), name, " is on ", t.device(), ", expected ", ref.device());
     return type_of(t, name);
 }
+inline int64_t rows_of(const Tensor& t) { return t.numel() / t.size(-1); }
 int need_param(const Tensor& t, const char* name, const Tensor& rows) {
     TORCH_CHECK(t.is_cuda() && t.device() == rows.device(), name, " is on ", t.device(), ", expected ", rows.device());
-    TORCH_CHECK(t.dim() == 1 && t.size(0) == rows.size(1) && t.is_contiguous(), name, " must be a contiguous vector of ",
-                rows.size(1), " elements, got shape ", t.sizes());
+    TORCH_CHECK(t.dim() == 1 && t.size(0) == rows.size(-1) && t.is_contiguous(), name, " must be a contiguous vector of ",
+                rows.size(-1), " elements, got shape ", t.sizes());
     return type_of(t, name);
 }
 
@@ -400,7 +404,7 @@ std::tuple<Tensor, OptTensor> dropout_add(const Tensor& x, const OptTensor& resi
     Draw d = draw_for(drops(p, "p"), ticket, x);
     Tensor y = residual.has_value() ? at::empty_like(*residual) : at::empty_like(x);
     if (x.numel() == 0) return {y, d.ticket.has_value() ? OptTensor(d.ticket->zero_()) : OptTensor()};
-    ok(t5vq_dropout_add(x.data_ptr(), xt, ptr<void>(residual), x.size(0), x.size(1), p, d.seed, d.offset, d.seed_dev,
+    ok(t5vq_dropout_add(x.data_ptr(), xt, ptr<void>(residual), rows_of(x), x.size(-1), p, d.seed, d.offset, d.seed_dev,
                         d.offset_dev, d.ticket_out, y.data_ptr(), yt, stream_of(x)),
        "dropout_add");
     return {y, d.ticket};
@@ -414,7 +418,7 @@ Tensor dropout_backward(const Tensor& g, double p, const OptTensor& ticket, std:
     const Draw d = draw_for(drops(p, "p"), ticket, g);
     Tensor out = at::empty(g.sizes(), dtype.has_value() ? g.options().dtype(*dtype) : g.options());
     if (g.numel() == 0) return out;
-    ok(t5vq_dropout_add(g.data_ptr(), gt, nullptr, g.size(0), g.size(1), p, 0, 0, d.seed_dev, d.offset_dev, nullptr,
+    ok(t5vq_dropout_add(g.data_ptr(), gt, nullptr, rows_of(g), g.size(-1), p, 0, 0, d.seed_dev, d.offset_dev, nullptr,
                         out.data_ptr(), type_of(out, "dtype"), stream_of(g)),
        "dropout_backward");
     return out;
@@ -430,7 +434,7 @@ std::tuple<Tensor, OptTensor, OptTensor, OptTensor, OptTensor> norm_forward(
     const int bt = branch.has_value() ? need_rows(*branch, "branch", hidden) : ht;
     if (bias.has_value())
         TORCH_CHECK(need_param(*bias, "bias", hidden) == wt, "bias must be of weight's type, ", weight.scalar_type());
-    const int64_t N = hidden.size(0), D = hidden.size(1);
+    const int64_t N = rows_of(hidden), D = hidden.size(-1);
     if (token_image.has_value()) {
         TORCH_CHECK(need(*token_image, "token_image", at::kByte).numel() >= t5vq_token_image_bytes(N, D),
                     "token_image smaller than t5vq_token_image_bytes(N, D)");
@@ -467,7 +471,7 @@ std::tuple<Tensor, OptTensor, OptTensor, OptTensor> norm_backward(
     const c10::DeviceGuard guard(h.device());
     const int ht = need_rows(h, "h", h), ot = need_rows(g_out, "g_out", h), wt = need_param(weight, "weight", h);
     if (g_sum.has_value()) TORCH_CHECK(need_rows(*g_sum, "g_sum", h) == ht, "g_sum must be of h's type, ", h.scalar_type());
-    const int64_t N = h.size(0), D = h.size(1);
+    const int64_t N = rows_of(h), D = h.size(-1);
     TORCH_CHECK(need(stats, "stats", at::kFloat, 2).size(0) == N && stats.size(1) == 2, "stats must be [", N, ", 2]");
     TORCH_CHECK(stats.device() == h.device(), "stats is on ", stats.device(), ", expected ", h.device());
     const bool any = drops(p, "p") || (drops(branch_p, "branch_p") && branch_dtype.has_value());
@@ -499,6 +503,122 @@ std::tuple<Tensor, OptTensor, OptTensor, OptTensor> norm_backward(
                           stream_of(h)),
        "norm_backward");
     return {gh, gb, gw, gbias};
+}
+
+// ---- the same with a gradient (t5vqvae_amd.norms): one dispatcher crossing forward, none of Python's backward ------------
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
+Tensor bare(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
+bool asks(const Tensor& t) { return t.defined() && t.requires_grad(); }
+bool asks(const OptTensor& t) { return t.has_value() && asks(*t); }
+
+// The gradients that a backward pass gives, for a pass that itself records a graph (create_graph): they look differentiable,
+// and differentiating them is refused -- there is no second derivative here, and none is silently taken as zero.
+variable_list once(variable_list grads) {
+    if (!at::GradMode::is_enabled()) return grads;
+    for (auto& g : grads)
+        if (g.defined()) g = g.detach().requires_grad_(true);
+    auto err = std::make_shared<torch::autograd::DelayedError>("t5vq: gradients of dropout and norm cannot be differentiated again",
+                                                               static_cast<int64_t>(grads.size()));
+    return (*err)(std::move(grads));
+}
+
+struct DropoutFunction : torch::autograd::Function<DropoutFunction> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& residual, double p, const OptTensor& ticket) {
+        auto [y, drawn] = dropout_add(x.contiguous(), residual.has_value() ? OptTensor(residual->contiguous()) : residual, p,
+                                      ticket);
+        ctx->save_for_backward({ticket.has_value() ? *ticket : bare(drawn)});
+        ctx->saved_data["p"] = p;
+        ctx->saved_data["type"] = x.scalar_type();
+        ctx->saved_data["residual"] = residual.has_value();
+        return y;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list g) {
+        const Tensor ticket = ctx->get_saved_variables()[0];
+        variable_list out(4);
+        if (ctx->needs_input_grad(0))
+            out[0] = dropout_backward(g[0].contiguous(), ctx->saved_data["p"].toDouble(), opt(ticket),
+                                      ctx->saved_data["type"].toScalarType());
+        if (ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(1)) out[1] = g[0];
+        return once(std::move(out));
+    }
+};
+
+Tensor dropout_autograd(const Tensor& x, const OptTensor& residual, double p, const OptTensor& ticket) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    if (at::GradMode::is_enabled() && (asks(x) || asks(residual))) return DropoutFunction::apply(x, residual, p, ticket);
+    return std::get<0>(
+        dropout_add(x.contiguous(), residual.has_value() ? OptTensor(residual->contiguous()) : residual, p, ticket));
+}
+
+// outputs of a norm as one list: out, sum with a branch, row norms on request
+variable_list norm_outputs(const std::tuple<Tensor, OptTensor, OptTensor, OptTensor, OptTensor>& r) {
+    variable_list v{std::get<0>(r)};
+    if (std::get<1>(r).has_value()) v.push_back(*std::get<1>(r));
+    if (std::get<3>(r).has_value()) v.push_back(*std::get<3>(r));
+    return v;
+}
+
+struct NormFunction : torch::autograd::Function<NormFunction> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& hidden, const OptTensor& branch, const Tensor& weight,
+                                 const OptTensor& bias, const OptTensor& ticket, int64_t kind, double eps, double branch_p,
+                                 double p, std::optional<at::ScalarType> out_dtype, bool row_norms,
+                                 const OptTensor& token_image) {
+        const Tensor h = hidden.contiguous();
+        const auto r = norm_forward(h, branch.has_value() ? OptTensor(branch->contiguous()) : branch, weight, bias, kind, eps,
+                                    branch_p, p, ticket, out_dtype, true, row_norms, token_image);
+        ctx->save_for_backward({branch.has_value() ? *std::get<1>(r) : h, weight, *std::get<2>(r),
+                                ticket.has_value() ? *ticket : bare(std::get<4>(r))});
+        ctx->saved_data["kind"] = kind;
+        ctx->saved_data["branch_p"] = branch_p;
+        ctx->saved_data["p"] = p;
+        ctx->saved_data["branch"] = branch.has_value() ? c10::IValue(branch->scalar_type()) : c10::IValue();
+        ctx->saved_data["bias"] = bias.has_value();
+        ctx->set_materialize_grads(false);
+        if (row_norms) ctx->mark_non_differentiable({*std::get<3>(r)});
+        return norm_outputs(r);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list g) {
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &h = saved[0], &weight = saved[1], &stats = saved[2], &ticket = saved[3];
+        const double branch_p = ctx->saved_data["branch_p"].toDouble();
+        const bool branch = !ctx->saved_data["branch"].isNone();
+        const auto branch_type = branch ? ctx->saved_data["branch"].toScalarType() : h.scalar_type();
+        // needs_input_grad counts the tensors that the call had: hidden, branch?, weight, bias?
+        const bool need_branch = branch && ctx->needs_input_grad(1), need_weight = ctx->needs_input_grad(branch ? 2 : 1);
+        const bool need_bias = ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(branch ? 3 : 2);
+        const Tensor g_sum = branch && g[1].defined() ? g[1].contiguous() : Tensor();
+        variable_list out(12);
+        if (!g[0].defined()) {                       // nothing came back through the norm: the sum's gradient only
+            if (ctx->needs_input_grad(0)) out[0] = g_sum;
+            if (need_branch && g_sum.defined()) out[1] = dropout_backward(g_sum, branch_p, opt(ticket), branch_type);
+            return once(std::move(out));
+        }
+        // without a dropout of the branch its gradient is the stream's, unless it is of another type
+        const bool same = branch_type == h.scalar_type() && !drops(branch_p, "branch_p");
+        const auto r = norm_backward(g[0].contiguous(), opt(g_sum), h, weight, stats, ctx->saved_data["kind"].toInt(), branch_p,
+                                     ctx->saved_data["p"].toDouble(), opt(ticket),
+                                     need_branch && !same ? std::optional<at::ScalarType>(branch_type) : std::nullopt,
+                                     need_weight, need_bias);
+        if (ctx->needs_input_grad(0)) out[0] = std::get<0>(r);
+        if (need_branch) out[1] = same ? std::get<0>(r) : *std::get<1>(r);
+        out[2] = bare(std::get<2>(r));
+        out[3] = bare(std::get<3>(r));
+        return once(std::move(out));
+    }
+};
+
+variable_list norm_autograd(const Tensor& hidden, const OptTensor& branch, const Tensor& weight, const OptTensor& bias,
+                            int64_t kind, double eps, double branch_p, double p, const OptTensor& ticket,
+                            std::optional<at::ScalarType> out_dtype, bool row_norms, const OptTensor& token_image) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    if (at::GradMode::is_enabled() && (asks(hidden) || asks(branch) || asks(weight) || asks(bias)))
+        return NormFunction::apply(hidden, branch, weight, bias, ticket, kind, eps, branch_p, p, out_dtype, row_norms,
+                                   token_image);
+    return norm_outputs(norm_forward(hidden.contiguous(), branch.has_value() ? OptTensor(branch->contiguous()) : branch, weight,
+                                     bias, kind, eps, branch_p, p, ticket, out_dtype, false, row_norms, token_image));
 }
 
 // Tensors that are not on a ROCm device: there is no CPU path, say so instead of the dispatcher's listing
@@ -538,6 +658,9 @@ TORCH_LIBRARY(t5vq, m) {
     m.def("norm_backward(Tensor g_out, Tensor? g_sum, Tensor h, Tensor weight, Tensor stats, int kind, float branch_p, "
           "float p, Tensor? ticket, ScalarType? branch_dtype, bool want_weight, bool want_bias) -> "
           "(Tensor, Tensor?, Tensor?, Tensor?)");
+    m.def("dropout(Tensor x, Tensor? residual, float p, Tensor? ticket=None) -> Tensor");
+    m.def("norm(Tensor hidden, Tensor? branch, Tensor weight, Tensor? bias, int kind, float eps, float branch_p, float p, "
+          "Tensor? ticket=None, ScalarType? out_dtype=None, bool row_norms=False, Tensor(a!)? token_image=None) -> Tensor[]");
 }
 
 TORCH_LIBRARY_IMPL(t5vq, CUDA, m) {   // ROCm devices carry the CUDA dispatch key in torch
@@ -554,11 +677,18 @@ TORCH_LIBRARY_IMPL(t5vq, CUDA, m) {   // ROCm devices carry the CUDA dispatch ke
     m.impl("dropout_backward", &dropout_backward);
     m.impl("norm_forward", &norm_forward);
     m.impl("norm_backward", &norm_backward);
+    m.impl("dropout", &dropout_autograd);      // below autograd (inference mode)
+    m.impl("norm", &norm_autograd);
+}
+
+TORCH_LIBRARY_IMPL(t5vq, AutogradCUDA, m) {
+    m.impl("dropout", &dropout_autograd);
+    m.impl("norm", &norm_autograd);
 }
 
 TORCH_LIBRARY_IMPL(t5vq, CPU, m) {
     for (const char* name : {"vq_forward", "vq_finalize", "vq_step", "ste_backward", "scatter_rows", "cosine_backward",
                              "distances", "one_hot", "code_sqnorms", "dropout_add", "dropout_backward", "norm_forward",
-                             "norm_backward"})
+                             "norm_backward", "dropout", "norm"})
         m.impl(name, torch::CppFunction::makeFromBoxedFunction<&no_cpu_path>());
 }

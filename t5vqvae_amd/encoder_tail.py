@@ -26,7 +26,7 @@ from __future__ import annotations
 import torch
 from torch import nn
 
-from . import norms, ops
+from . import ops
 
 
 class _TailFunction(torch.autograd.Function):
@@ -107,14 +107,16 @@ class EncoderTailVQ(nn.Module):
         return self.vq(x.view(hidden_states.shape), srl, _xx=xx, _ximg=ximg if ximg.numel() else None)
 
     def _forward_counter(self, hidden_states, srl, branch, ticket):
-        rows = norms._rows(hidden_states, "hidden_states")
-        add = None if branch is None else norms._rows(branch, "branch", hidden_states)
-        n, d = rows.shape
+        d = hidden_states.shape[-1]
+        n = hidden_states.numel() // d if d else 0
         p, branch_p = (self.dropout_rate, self.branch_dropout_rate) if self.training else (0.0, 0.0)
-        ximg = ops.token_image(n, d, rows.device) if self._wants_image(n, d, srl) else None
-        x, _, xx = norms._norm_call(rows, add, self.weight, self.bias, self.norm, float(self.variance_epsilon), branch_p, p,
-                                    ticket, torch.float32, row_norms=True, token_image=ximg)
-        return self.vq(x.view(hidden_states.shape), srl, _xx=xx, _ximg=ximg)
+        ximg = None
+        if hidden_states.is_cuda and self._wants_image(n, d, srl):
+            ximg = ops.token_image(n, d, hidden_states.device)
+        x, *_, xx = ops.norm(hidden_states, branch, self.weight, self.bias, kind=self.norm, eps=self.variance_epsilon,
+                             branch_p=branch_p, p=p, ticket=ticket, out_dtype=torch.float32, row_norms=True,
+                             token_image=ximg)
+        return self.vq(x, srl, _xx=xx, _ximg=ximg)
 
     def _wants_image(self, n: int, d: int, srl) -> bool:
         """Whether the quantizer's search of this call will be the filtered one in token order -- then the norm kernel

@@ -668,6 +668,13 @@ def norm_forward(hidden, weight, bias=None, *, kind: str = "layer", eps: float =
                                               out_dtype, want_stats, want_row_norms, token_image)
 
 
+def norm(hidden, branch, weight, bias, *, kind: str, eps: float, branch_p: float, p: float, ticket=None, out_dtype=None,
+         row_norms: bool = False, token_image=None):
+    """[out, sum (with a branch), xx (with ``row_norms``)] with a gradient where one is wanted: t5vq::norm."""
+    return _lib.load_torch_ops().norm.default(hidden, branch, weight, bias, _norm_kind(kind), eps, branch_p, p, ticket,
+                                              out_dtype, row_norms, token_image)
+
+
 def norm_backward(g_out, g_sum, h, weight, stats, *, kind: str = "layer", branch_p: float = 0.0, p: float = 0.0, ticket=None,
                   branch_dtype=None, want_weight: bool = True, want_bias: bool = True):
     """(grad_hidden, grad_branch | None, grad_weight | None, grad_bias | None): t5vq::norm_backward.  ``h``: the rows that
