@@ -19,25 +19,32 @@ template <> struct Group<float> { typedef float type __attribute__((ext_vector_t
 template <> struct Group<__bf16> { typedef __bf16 type __attribute__((ext_vector_type(4), aligned(2))); };
 template <> struct Group<_Float16> { typedef _Float16 type __attribute__((ext_vector_type(4), aligned(2))); };
 
-// columns c .. c + 3 of a row of D elements; columns >= D read as 0
-template <class T>
-__device__ __forceinline__ f32x4 load_group(const T* __restrict__ row, int c, int D) {
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    if (c + 4 <= D) {
-        v = __builtin_convertvector(*reinterpret_cast<const typename Group<T>::type*>(row + c), f32x4);
-    } else if (c < D) {
-        v.x = static_cast<float>(row[c]);
-        if (c + 1 < D) v.y = static_cast<float>(row[c + 1]);
-        if (c + 2 < D) v.z = static_cast<float>(row[c + 2]);
+// Columns c .. c + 3 of a row of D elements, as they are in memory; columns >= D read as 0.  FULL: there are none (a row that
+// fills every lane's groups: no comparison, no branch).
+template <bool FULL, class T>
+__device__ __forceinline__ typename Group<T>::type load_raw(const T* __restrict__ row, unsigned c, unsigned D) {
+    typedef typename Group<T>::type V;
+    if (FULL || c + 4 <= D) return *reinterpret_cast<const V*>(row + c);
+    V v = {T(0), T(0), T(0), T(0)};
+    if (c < D) {
+        v.x = row[c];
+        if (c + 1 < D) v.y = row[c + 1];
+        if (c + 2 < D) v.z = row[c + 2];
     }
     return v;
 }
+template <class V>
+__device__ __forceinline__ f32x4 widen(V v) { return __builtin_convertvector(v, f32x4); }
+template <bool FULL = false, class T>
+__device__ __forceinline__ f32x4 load_group(const T* __restrict__ row, unsigned c, unsigned D) {
+    return widen(load_raw<FULL>(row, c, D));
+}
 // each value rounded once, to nearest even
-template <class T>
-__device__ __forceinline__ void store_group(T* __restrict__ row, int c, int D, f32x4 v) {
-    if (c + 4 <= D) {
-        typedef typename Group<T>::type G;
-        *reinterpret_cast<G*>(row + c) = __builtin_convertvector(v, G);
+template <bool FULL = false, class T>
+__device__ __forceinline__ void store_group(T* __restrict__ row, unsigned c, unsigned D, f32x4 v) {
+    if (FULL || c + 4 <= D) {
+        typedef typename Group<T>::type V;
+        *reinterpret_cast<V*>(row + c) = __builtin_convertvector(v, V);
     } else if (c < D) {
         row[c] = static_cast<T>(v.x);
         if (c + 1 < D) row[c + 1] = static_cast<T>(v.y);
@@ -50,7 +57,7 @@ __device__ __forceinline__ f32x4 round_group(f32x4 v) {   // what a later read o
     return __builtin_convertvector(__builtin_convertvector(v, V), f32x4);
 }
 // a parameter vector whose type is only known at run time (its reads are few: once per row at most, from cache)
-__device__ __forceinline__ f32x4 load_param(const void* p, int type, int c, int D) {
+__device__ __forceinline__ f32x4 load_param(const void* p, int type, unsigned c, unsigned D) {
     if (type == T5VQ_F32) return load_group(static_cast<const float*>(p), c, D);
     if (type == T5VQ_BF16) return load_group(static_cast<const __bf16*>(p), c, D);
     return load_group(static_cast<const _Float16*>(p), c, D);
@@ -100,9 +107,9 @@ __device__ __forceinline__ Words philox(const Key k, unsigned block, unsigned ro
     for (int i = 0; i < 10; ++i) {
         const unsigned long long u = static_cast<unsigned long long>(a) * 0xD2511F53u;
         const unsigned long long v = static_cast<unsigned long long>(c) * 0xCD9E8D57u;
-        a = static_cast<unsigned>(v >> 32) ^ b ^ k0;
+        a = __builtin_amdgcn_bitop3_b32(static_cast<unsigned>(v >> 32), b, k0, 0x96);   // x ^ y ^ z
         b = static_cast<unsigned>(v);
-        c = static_cast<unsigned>(u >> 32) ^ d ^ k1;
+        c = __builtin_amdgcn_bitop3_b32(static_cast<unsigned>(u >> 32), d, k1, 0x96);
         d = static_cast<unsigned>(u);
         k0 += 0x9E3779B9u;
         k1 += 0xBB67AE85u;
@@ -110,23 +117,43 @@ __device__ __forceinline__ Words philox(const Key k, unsigned block, unsigned ro
     return {a, b, c, d};
 }
 // A dropped element is 0 whatever it held (an infinity or NaN included).
-__device__ __forceinline__ f32x4 drop_group(f32x4 v, unsigned lo, unsigned hi, Drop d) {
-    v.x = (lo & 0xFFFFu) < d.kept ? v.x * d.scale : 0.f;
-    v.y = (lo >> 16) < d.kept ? v.y * d.scale : 0.f;
-    v.z = (hi & 0xFFFFu) < d.kept ? v.z * d.scale : 0.f;
-    v.w = (hi >> 16) < d.kept ? v.w * d.scale : 0.f;
+__device__ __forceinline__ f32x4 keep_group(f32x4 v, unsigned lo, unsigned hi, unsigned kept) {
+    v.x = (lo & 0xFFFFu) < kept ? v.x : 0.f;
+    v.y = (lo >> 16) < kept ? v.y : 0.f;
+    v.z = (hi & 0xFFFFu) < kept ? v.z : 0.f;
+    v.w = (hi >> 16) < kept ? v.w : 0.f;
     return v;
+}
+__device__ __forceinline__ f32x4 drop_group(f32x4 v, unsigned lo, unsigned hi, Drop d) {
+    return keep_group(v * d.scale, lo, hi, d.kept);
 }
 __device__ __forceinline__ f32x4 drop_at(f32x4 v, Key k, int q, unsigned row, Drop d) {   // group q of a row, by itself
     const Words w = philox(k, static_cast<unsigned>(q) >> 1, row);
     return (q & 1) ? drop_group(v, w.w2, w.w3, d) : drop_group(v, w.w0, w.w1, d);
 }
 
-__device__ __forceinline__ float wave_sum(float v) {   // xor butterfly: the order every row norm of the library uses
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+// Sum over G = 16 or 64 neighbouring lanes, in every one of them: the xor butterfly from the widest step down -- the order
+// every row norm of the library uses -- made of register moves alone (no LDS permutes): v_permlane32/16_swap, DPP rotations
+// and shifts.
+template <int G>
+__device__ __forceinline__ float lanes_sum(float v) {
+    auto moved = [](float x, auto f) { return __int_as_float(f(__float_as_int(x))); };
+    if constexpr (G > 16) {
+        const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+        const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(b[0]) + __uint_as_float(b[1]);
+    }
+    v += moved(v, [](int x) { return __builtin_amdgcn_update_dpp(0, x, 0x128, 0xF, 0xF, false); });        // row_ror:8
+    v += moved(v, [](int x) {                                                                             // lane ^ 4
+        const int up = __builtin_amdgcn_update_dpp(0, x, 0x104, 0xF, 0x5, false);                          // row_shl:4
+        return __builtin_amdgcn_update_dpp(up, x, 0x114, 0xF, 0xA, false);                                 // row_shr:4
+    });
+    v += moved(v, [](int x) { return __builtin_amdgcn_update_dpp(0, x, 0x4E, 0xF, 0xF, false); });         // quad_perm: lane ^ 2
+    v += moved(v, [](int x) { return __builtin_amdgcn_update_dpp(0, x, 0xB1, 0xF, 0xF, false); });         // quad_perm: lane ^ 1
     return v;
 }
+__device__ __forceinline__ float wave_sum(float v) { return lanes_sum<64>(v); }
 __device__ __forceinline__ float sq4(const f32x4 v, float s) {
     s = fmaf(v.x, v.x, s);
     s = fmaf(v.y, v.y, s);
@@ -134,32 +161,51 @@ __device__ __forceinline__ float sq4(const f32x4 v, float s) {
     s = fmaf(v.w, v.w, s);
     return s;
 }
+__device__ __forceinline__ f32x4 fma4(const f32x4 a, const f32x4 b, const f32x4 c) {
+    return f32x4{fmaf(a.x, b.x, c.x), fmaf(a.y, b.y, c.y), fmaf(a.z, b.z, c.z), fmaf(a.w, b.w, c.w)};
+}
 __device__ __forceinline__ float sum4(const f32x4 v, float s) { return s + ((v.x + v.y) + (v.z + v.w)); }
 
-// The dropout of a row held in registers, group lane + G * j in v[j] (G >= 2 lanes a row, G even).  Neighbouring lanes hold
-// the two halves of a block; for two chunks j, j + 1 the even lane draws chunk j's block and the odd lane chunk j + 1's, and
-// each hands its neighbour the two words it needs: half the draws of every lane drawing for itself.
-template <int G, int NCH>
-__device__ __forceinline__ void drop_row(f32x4 (&v)[NCH], Key k, unsigned row, int lane, Drop d) {
+// Draws for a row held in registers, group lane + G * j in chunk j (G even).  Neighbouring lanes hold the two halves of a
+// block; for two chunks j, j + 1 the even lane draws chunk j's block and the odd lane chunk j + 1's, and each hands its
+// neighbour the two words it needs: half the draws of every lane drawing for itself.  f(j, lo, hi) gets chunk j's bits.
+template <int G, int NCH, class F>
+__device__ __forceinline__ void row_draws(Key k, unsigned row, unsigned lane, F f) {
     const bool odd = lane & 1;
 #pragma unroll
     for (int j = 0; j + 1 < NCH; j += 2) {
-        const Words w = philox(k, static_cast<unsigned>(lane + G * (odd ? j + 1 : j)) >> 1, row);
+        const Words w = philox(k, ((lane >> 1) + (G / 2) * j) + (odd ? G / 2 : 0), row);
         const unsigned s0 = odd ? w.w0 : w.w2, s1 = odd ? w.w1 : w.w3;      // the neighbour's half of my block
         const unsigned m0 = odd ? w.w2 : w.w0, m1 = odd ? w.w3 : w.w1;      // mine
         const unsigned r0 = __builtin_amdgcn_mov_dpp(s0, 0xB1, 0xF, 0xF, true);   // quad_perm [1, 0, 3, 2]
         const unsigned r1 = __builtin_amdgcn_mov_dpp(s1, 0xB1, 0xF, 0xF, true);
-        v[j] = drop_group(v[j], odd ? r0 : m0, odd ? r1 : m1, d);
-        v[j + 1] = drop_group(v[j + 1], odd ? m0 : r0, odd ? m1 : r1, d);
+        f(j, odd ? r0 : m0, odd ? r1 : m1);
+        f(j + 1, odd ? m0 : r0, odd ? m1 : r1);
     }
-    if constexpr (NCH & 1) v[NCH - 1] = drop_at(v[NCH - 1], k, lane + G * (NCH - 1), row, d);
+    if constexpr (NCH & 1) {
+        const Words w = philox(k, (lane >> 1) + (G / 2) * (NCH - 1), row);
+        f(NCH - 1, odd ? w.w2 : w.w0, odd ? w.w3 : w.w1);
+    }
 }
 
-// sum over the G lanes of a row (G: a multiple of 64), fixed order; slots: G / 64 floats of LDS, and one more set for the
+// where a thread stands: G lanes a row, a workgroup of at least 256 threads.  With a row to every wave or more the row is the
+// wave's, and kept in scalar registers.
+template <int G>
+struct Place {
+    static constexpr int WG = G > 256 ? G : 256, ROWS = WG / G;
+    unsigned lane, sub;
+    __device__ __forceinline__ Place() {
+        lane = threadIdx.x & (G - 1);
+        sub = threadIdx.x / G;
+        if constexpr (G >= 64) sub = __builtin_amdgcn_readfirstlane(sub);
+    }
+};
+
+// sum over the G lanes of a row (16, or a multiple of 64), fixed order; slots: G / 64 floats of LDS, and one more set for the
 // next call, which may then write before every wave has read this one's
 template <int G>
 __device__ __forceinline__ float row_sum(float v, float* slots) {
-    v = wave_sum(v);
+    v = lanes_sum<(G < 64 ? G : 64)>(v);
     if constexpr (G > 64) {
         if ((threadIdx.x & 63) == 0) slots[threadIdx.x >> 6] = v;
         __syncthreads();
@@ -170,14 +216,31 @@ __device__ __forceinline__ float row_sum(float v, float* slots) {
     return v;
 }
 // values of columns >= D to 0 (they only exist in a row's last group and behind it)
-__device__ __forceinline__ f32x4 inside(f32x4 v, int c, int D) {
-    if (c + 4 > D) {
+template <bool FULL>
+__device__ __forceinline__ f32x4 inside(f32x4 v, unsigned c, unsigned D) {
+    if (!FULL && c + 4 > D) {
         if (c >= D) v.x = 0.f;
         if (c + 1 >= D) v.y = 0.f;
         if (c + 2 >= D) v.z = 0.f;
         v.w = 0.f;
     }
     return v;
+}
+
+// Workgroups that walk N rows, `rows` at a time each: as many as the card holds at once, fewer where each then walks equally
+// many rows.
+template <class K>
+inline int64_t resident(K kernel, int threads) {   // of one kernel on one CU; asked once a kernel
+    int n = 0;
+    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, 0) != hipSuccess || n < 1) n = 1;
+    return n;
+}
+constexpr int64_t CUS = 256;
+inline int64_t workgroups(int64_t N, int64_t rows, int64_t most) {
+    const int64_t wgs = (N + rows - 1) / rows;
+    if (wgs <= most) return wgs;
+    const int64_t turns = (wgs + most - 1) / most;
+    return (wgs + turns - 1) / turns;
 }
 
 inline bool known_type(int t) { return t == T5VQ_F32 || t == T5VQ_BF16 || t == T5VQ_F16; }

@@ -50,38 +50,55 @@ struct NormArgs {
 };
 
 // A row in registers: G lanes hold it, group lane + G * j in chunk j of NCH.  One read of each input, one write of each
-// output; G = 64 (one wave a row, no barrier) up to 2048 columns, a workgroup a row above.  The parameters stay in registers
-// while a wave walks its rows.
-template <class TH, class TB, class TO, bool ADD, int G, int NCH>
-__global__ __launch_bounds__(G > 256 ? G : 256) void norm_kernel(const TH* __restrict__ hidden, const TB* __restrict__ branch,
-                                                                 TO* __restrict__ out, TH* __restrict__ sum, NormArgs a) {
-    constexpr int WG = G > 256 ? G : 256, ROWS = WG / G;
+// output; G = 16 (four rows a wave) or 64 (one) without a barrier, a workgroup a row above.  The parameters stay in registers
+// while a wave walks its rows, and the next row is on its way while this one is worked on.  FULL: D = 4 G NCH.
+template <class TH, class TB, class TO, bool ADD, int G, int NCH, bool FULL>
+__global__ __launch_bounds__(Place<G>::WG) void norm_kernel(const TH* __restrict__ hidden, const TB* __restrict__ branch,
+                                                            TO* __restrict__ out, TH* __restrict__ sum, NormArgs a) {
+    constexpr int ROWS = Place<G>::ROWS;
     __shared__ float slots[2][G > 64 ? G / 64 : 1];
-    const int lane = threadIdx.x & (G - 1), D = a.D;
+    __shared__ f32x4 copy[std::is_same<TO, float>::value && G == 256 && NCH == 2 ? G * NCH : 1];
+    const Place<G> at;
+    const unsigned lane = at.lane, D = FULL ? 4 * G * NCH : a.D;
     if (a.ctr.ticket_out && blockIdx.x == 0 && threadIdx.x == 0) give_ticket(a.ctr);
     const Key k0 = site_key(a.ctr, 0), k1 = site_key(a.ctr, 1);
     const f32x4 zero4 = {0.f, 0.f, 0.f, 0.f};
-    f32x4 w[NCH], b[NCH];
+    f32x4 w[NCH], b[NCH];           // times the output's scale: a kept value needs no multiplication of its own
 #pragma unroll
     for (int j = 0; j < NCH; ++j) {
-        w[j] = load_param(a.weight, a.weight_type, 4 * (lane + G * j), D);
-        b[j] = a.bias ? load_param(a.bias, a.weight_type, 4 * (lane + G * j), D) : zero4;
+        w[j] = load_param(a.weight, a.weight_type, 4 * (lane + G * j), D) * a.out.scale;
+        b[j] = a.bias ? load_param(a.bias, a.weight_type, 4 * (lane + G * j), D) * a.out.scale : zero4;
     }
     const float inv_d = 1.0f / static_cast<float>(D);
-    for (long long row = static_cast<long long>(blockIdx.x) * ROWS + threadIdx.x / G; row < a.N;
-         row += static_cast<long long>(gridDim.x) * ROWS) {
-        f32x4 h[NCH];
+    const long long step = static_cast<long long>(gridDim.x) * ROWS;
+    long long row = static_cast<long long>(blockIdx.x) * ROWS + at.sub;
+    typename Group<TH>::type hn[NCH];
+    typename Group<TB>::type bn[NCH];
+    auto fetch = [&](long long r) {
 #pragma unroll
-        for (int j = 0; j < NCH; ++j) h[j] = load_group(hidden + row * D, 4 * (lane + G * j), D);
+        for (int j = 0; j < NCH; ++j) {
+            hn[j] = load_raw<FULL>(hidden + r * D, 4 * (lane + G * j), D);
+            if constexpr (ADD) bn[j] = load_raw<FULL>(branch + r * D, 4 * (lane + G * j), D);
+        }
+    };
+    if (row < a.N) fetch(row);
+    for (; row < a.N; row += step) {
+        f32x4 h[NCH], br[ADD ? NCH : 1];
+#pragma unroll
+        for (int j = 0; j < NCH; ++j) {
+            h[j] = widen(hn[j]);
+            if constexpr (ADD) br[j] = widen(bn[j]);
+        }
+        if (row + step < a.N) fetch(row + step);
         if constexpr (ADD) {
-            f32x4 br[NCH];
-#pragma unroll
-            for (int j = 0; j < NCH; ++j) br[j] = load_group(branch + row * D, 4 * (lane + G * j), D);
-            if (a.branch.kept < 65536u) drop_row<G>(br, k0, static_cast<unsigned>(row), lane, a.branch);
+            if (a.branch.kept < 65536u)
+                row_draws<G, NCH>(k0, static_cast<unsigned>(row), lane, [&](int j, unsigned lo, unsigned hi) {
+                    br[j] = drop_group(br[j], lo, hi, a.branch);
+                });
 #pragma unroll
             for (int j = 0; j < NCH; ++j) {
                 h[j] = round_group<TH>(h[j] + br[j]);
-                store_group(sum + row * D, 4 * (lane + G * j), D, h[j]);
+                store_group<FULL>(sum + row * D, 4 * (lane + G * j), D, h[j]);
             }
         }
         float mean = 0.f, s = 0.f;
@@ -93,7 +110,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void norm_kernel(const TH* __res
         }
 #pragma unroll
         for (int j = 0; j < NCH; ++j) {
-            h[j] = inside(h[j] - mean, 4 * (lane + G * j), D);
+            h[j] = inside<FULL>(h[j] - mean, 4 * (lane + G * j), D);
             s = sq4(h[j], s);
         }
         const float r = 1.0f / __fsqrt_rn(row_sum<G>(s, slots[1]) * inv_d + a.eps);
@@ -102,33 +119,47 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void norm_kernel(const TH* __res
             a.stats[2 * row + 1] = r;
         }
 #pragma unroll
-        for (int j = 0; j < NCH; ++j) h[j] = h[j] * r * w[j] + b[j];
-        if (a.out.kept < 65536u) drop_row<G>(h, k1, static_cast<unsigned>(row), lane, a.out);
-        float m = 0.f;
-        s = 0.f;
+        for (int j = 0; j < NCH; ++j) h[j] = fma4(h[j] * r, w[j], b[j]);
+        if (a.out.kept < 65536u)
+            row_draws<G, NCH>(k1, static_cast<unsigned>(row), lane, [&](int j, unsigned lo, unsigned hi) {
+                h[j] = keep_group(h[j], lo, hi, a.out.kept);
+            });
 #pragma unroll
-        for (int j = 0; j < NCH; ++j) {
-            store_group(out + row * D, 4 * (lane + G * j), D, h[j]);
-            if (std::is_same<TO, float>::value && G == 64) {
-                s = sq4(h[j], s);
-                m = t5vq_absmax4(m, h[j].x, h[j].y, h[j].z, h[j].w);
-            }
-        }
-        if constexpr (std::is_same<TO, float>::value && G == 64) {   // what the searches take of fp32 rows (D <= 2048)
-            if (a.xx) {
-                s = wave_sum(s);
-                if (lane == 0) a.xx[row] = s;
-            }
-            if (a.img.rows) {
+        for (int j = 0; j < NCH; ++j) store_group<FULL>(out + row * D, 4 * (lane + G * j), D, h[j]);
+        if constexpr (std::is_same<TO, float>::value && 4 * G * NCH <= 2048) {   // what the searches take of fp32 rows
+            if (a.xx || a.img.rows) {
+                float m = 0.f, inv;
+                s = 0.f;
+                if constexpr (G <= 64) {
 #pragma unroll
-                for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-                float inv;
-                const float sc = t5vq_image_scale(m, &inv);
-                if (lane == 0) a.img.inv[row] = inv;
+                    for (int j = 0; j < NCH; ++j) {
+                        // 16 lanes: the groups of a second chunk belong to a wave's lanes 16 .. 31, a chain of their own
+                        s = G < 64 ? s + sq4(h[j], 0.f) : sq4(h[j], s);
+                        m = t5vq_absmax4(m, h[j].x, h[j].y, h[j].z, h[j].w);
+                    }
+                } else {   // a row's norm is defined on one wave's lanes: through LDS, every wave adds all of it
 #pragma unroll
-                for (int j = 0; j < NCH; ++j) {
-                    const int q = lane + G * j;
-                    if (4 * q < D) t5vq_image_store4(a.img.rows + row * D, q, h[j].x, h[j].y, h[j].z, h[j].w, sc);
+                    for (int j = 0; j < NCH; ++j) copy[lane + G * j] = h[j];
+                    __syncthreads();
+#pragma unroll
+                    for (int q = 0; q < G * NCH; q += 64) {
+                        const f32x4 v = copy[(lane & 63) + q];
+                        s = sq4(v, s);
+                        m = t5vq_absmax4(m, v.x, v.y, v.z, v.w);
+                    }
+                }
+                s = lanes_sum<(G < 64 ? G : 64)>(s);
+                if (a.xx && lane == 0) a.xx[row] = s;
+                if (a.img.rows) {
+#pragma unroll
+                    for (int o = (G < 64 ? G : 64) / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+                    const float sc = t5vq_image_scale(m, &inv);
+                    if (lane == 0) a.img.inv[row] = inv;
+#pragma unroll
+                    for (int j = 0; j < NCH; ++j) {
+                        const unsigned q = lane + G * j;
+                        if (4 * q < D) t5vq_image_store4(a.img.rows + row * D, q, h[j].x, h[j].y, h[j].z, h[j].w, sc);
+                    }
                 }
             }
         }
@@ -193,30 +224,33 @@ __global__ __launch_bounds__(256) void norm_rows_kernel(const TH* __restrict__ h
     }
 }
 
-constexpr int64_t MOST_WGS = 2048;   // 256 CUs x 8 workgroups of four waves: what is resident at 64 registers
+template <class TH, class TB, class TO, bool ADD, int G, int NCH, bool FULL>
+void go(const void* hidden, const void* branch, void* out, void* sum, const NormArgs& a, hipStream_t stream) {
+    constexpr auto kernel = norm_kernel<TH, TB, TO, ADD, G, NCH, FULL>;
+    constexpr int threads = Place<G>::WG;
+    static const int64_t most = CUS * resident(kernel, threads);
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(workgroups(a.N, Place<G>::ROWS, most))), dim3(threads), 0, stream,
+                       static_cast<const TH*>(hidden), static_cast<const TB*>(branch), static_cast<TO*>(out),
+                       static_cast<TH*>(sum), a);
+}
 
 template <class TH, class TB, class TO, bool ADD>
-void launch_norm(const void* hidden, const void* branch, void* out, void* sum, int64_t N, const NormArgs& a,
-                 hipStream_t stream) {
-#define T5VQ_NK(G, NCH)                                                                                                     \
-    do {                                                                                                                    \
-        constexpr int64_t rows = G >= 256 ? 1 : 256 / G;                                                                    \
-        const int64_t wgs = (N + rows - 1) / rows;                                                                          \
-        hipLaunchKernelGGL((norm_kernel<TH, TB, TO, ADD, G, NCH>),                                                          \
-                           dim3(static_cast<unsigned>(wgs < MOST_WGS ? wgs : MOST_WGS)), dim3(G > 256 ? G : 256), 0, stream, \
-                           static_cast<const TH*>(hidden), static_cast<const TB*>(branch), static_cast<TO*>(out),           \
-                           static_cast<TH*>(sum), a);                                                                       \
-    } while (0)
-    if (a.D <= 256) T5VQ_NK(64, 1);
+void launch_norm(const void* hidden, const void* branch, void* out, void* sum, const NormArgs& a, hipStream_t stream) {
+#define T5VQ_NK(G, NCH)                                                                                        \
+    (a.D == 4 * G * NCH ? go<TH, TB, TO, ADD, G, NCH, true>(hidden, branch, out, sum, a, stream)               \
+                        : go<TH, TB, TO, ADD, G, NCH, false>(hidden, branch, out, sum, a, stream))
+    if (a.D <= 64) T5VQ_NK(16, 1);
+    else if (a.D <= 128) T5VQ_NK(16, 2);
+    else if (a.D <= 256) T5VQ_NK(64, 1);
     else if (a.D <= 512) T5VQ_NK(64, 2);
     else if (a.D <= 768) T5VQ_NK(64, 3);
     else if (a.D <= 1024) T5VQ_NK(64, 4);
-    else if (a.D <= 2048) T5VQ_NK(64, 8);
+    else if (a.D <= 2048) T5VQ_NK(256, 2);
     else if (a.D <= 4096) T5VQ_NK(256, 4);
     else if (a.D <= 8192) T5VQ_NK(1024, 2);
     else if (a.D <= 16384) T5VQ_NK(1024, 4);
     else
-        hipLaunchKernelGGL((norm_rows_kernel<TH, TB, TO, ADD>), dim3(static_cast<unsigned>(N < MOST_WGS ? N : MOST_WGS)),
+        hipLaunchKernelGGL((norm_rows_kernel<TH, TB, TO, ADD>), dim3(static_cast<unsigned>(workgroups(a.N, 1, CUS * 8))),
                            dim3(256), 0, stream, static_cast<const TH*>(hidden), static_cast<const TB*>(branch),
                            static_cast<TO*>(out), static_cast<TH*>(sum), a);
 #undef T5VQ_NK
@@ -305,7 +339,7 @@ int t5vq_norm_forward(const void* hidden, int hidden_type, const void* branch, i
              reinterpret_cast<long long*>(ticket_out)};
     a.stats = stats, a.xx = xx, a.img = t5vq_token_image_parts(token_image, N, D);
     hipStream_t s = static_cast<hipStream_t>(stream);
-#define T5VQ_NF(H, B, O, ADD) launch_norm<H, B, O, ADD>(hidden, branch, out, sum, N, a, s)
+#define T5VQ_NF(H, B, O, ADD) launch_norm<H, B, O, ADD>(hidden, branch, out, sum, a, s)
 #define T5VQ_NF_HALF(H)                                                                         \
     (out_type == T5VQ_F32 ? (branch ? T5VQ_NF(H, H, float, true) : T5VQ_NF(H, H, float, false)) \
                           : (branch ? T5VQ_NF(H, H, H, true) : T5VQ_NF(H, H, H, false)))

@@ -29,71 +29,105 @@ __device__ __forceinline__ float block_sum(float v, float* slots) {   // 256 thr
 //   grad_weight = sum over rows of gy n, grad_bias = sum of gy.
 // The row stays in registers between its two sums and its gradients (group lane + G * j in chunk j, as forward), and a wave
 // adds up the parameters' gradients of all rows it walks: every input is read once.  Workgroup b leaves its sums in part[b].
-template <class TO, class TH, class TB, int G, int NCH>
-__global__ __launch_bounds__(G > 256 ? G : 256) void norm_backward_kernel(const TO* __restrict__ g,
-                                                                          const TH* __restrict__ g_sum,
-                                                                          const TH* __restrict__ h, BackArgs a,
-                                                                          TH* __restrict__ grad_h,
-                                                                          TB* __restrict__ grad_branch,
-                                                                          float* __restrict__ part) {
-    constexpr int WG = G > 256 ? G : 256, ROWS = WG / G;
+template <class TO, class TH, class TB, int G, int NCH, bool FULL>
+__global__ __launch_bounds__(Place<G>::WG) void norm_backward_kernel(const TO* __restrict__ g, const TH* __restrict__ g_sum,
+                                                                     const TH* __restrict__ h, BackArgs a,
+                                                                     TH* __restrict__ grad_h, TB* __restrict__ grad_branch,
+                                                                     float* __restrict__ part) {
+    constexpr int ROWS = Place<G>::ROWS;
     __shared__ float slots[2][G > 64 ? G / 64 : 1];
     __shared__ f32x4 sums[ROWS > 1 ? ROWS : 1][ROWS > 1 ? G * NCH : 1];
-    const int lane = threadIdx.x & (G - 1), D = a.D;
+    const Place<G> at;
+    const unsigned lane = at.lane, D = FULL ? 4 * G * NCH : a.D;
     const Key k0 = site_key(a.ctr, 0), k1 = site_key(a.ctr, 1);
     const f32x4 zero4 = {0.f, 0.f, 0.f, 0.f};
-    f32x4 w[NCH], gw[NCH], gb[NCH];
+    f32x4 w[NCH], gw[NCH], gb[NCH];   // w times the output's scale; gw, gb without it until the end
 #pragma unroll
     for (int j = 0; j < NCH; ++j) {
-        w[j] = load_param(a.weight, a.weight_type, 4 * (lane + G * j), D);
+        w[j] = load_param(a.weight, a.weight_type, 4 * (lane + G * j), D) * a.out.scale;
         gw[j] = zero4;
         gb[j] = zero4;
     }
     const float inv_d = 1.0f / static_cast<float>(D);
-    for (long long row = static_cast<long long>(blockIdx.x) * ROWS + threadIdx.x / G; row < a.N;
-         row += static_cast<long long>(gridDim.x) * ROWS) {
-        f32x4 v[NCH], n[NCH], gs[NCH];
+    const long long step = static_cast<long long>(gridDim.x) * ROWS;
+    long long row = static_cast<long long>(blockIdx.x) * ROWS + at.sub;
+    typename Group<TO>::type vn[NCH];
+    typename Group<TH>::type nn[NCH], sn[NCH];
+    float mean_n = 0.f, r_n = 0.f;
+    auto fetch = [&](long long t) {
 #pragma unroll
         for (int j = 0; j < NCH; ++j) {
-            v[j] = load_group(g + row * D, 4 * (lane + G * j), D);
-            n[j] = load_group(h + row * D, 4 * (lane + G * j), D);
-            gs[j] = g_sum ? load_group(g_sum + row * D, 4 * (lane + G * j), D) : zero4;
+            vn[j] = load_raw<FULL>(g + t * D, 4 * (lane + G * j), D);
+            nn[j] = load_raw<FULL>(h + t * D, 4 * (lane + G * j), D);
         }
-        const float mean = a.stats[2 * row], r = a.stats[2 * row + 1];
-        if (a.out.kept < 65536u) drop_row<G>(v, k1, static_cast<unsigned>(row), lane, a.out);
+        if (g_sum) {
+#pragma unroll
+            for (int j = 0; j < NCH; ++j) sn[j] = load_raw<FULL>(g_sum + t * D, 4 * (lane + G * j), D);
+        }
+        mean_n = a.stats[2 * t];
+        r_n = a.stats[2 * t + 1];
+    };
+    if (row < a.N) fetch(row);
+    for (; row < a.N; row += step) {
+        f32x4 v[NCH], n[NCH];
+        typename Group<TH>::type gs[NCH];
+#pragma unroll
+        for (int j = 0; j < NCH; ++j) {
+            v[j] = widen(vn[j]);
+            n[j] = widen(nn[j]);
+            gs[j] = sn[j];
+        }
+        const float mean = mean_n, r = r_n;
+        if (row + step < a.N) fetch(row + step);
+        if (a.out.kept < 65536u)
+            row_draws<G, NCH>(k1, static_cast<unsigned>(row), lane, [&](int j, unsigned lo, unsigned hi) {
+                v[j] = keep_group(v[j], lo, hi, a.out.kept);
+            });
         float s1 = 0.f, s2 = 0.f;
 #pragma unroll
         for (int j = 0; j < NCH; ++j) {
             n[j] = (n[j] - mean) * r;      // behind the row's end g is 0: what n is there reaches no sum
-            gw[j] += v[j] * n[j];
+            gw[j] = fma4(v[j], n[j], gw[j]);
             gb[j] += v[j];
             v[j] *= w[j];
             s1 = sum4(v[j], s1);
-            s2 = sum4(v[j] * n[j], s2);
+            s2 = fmaf(v[j].x, n[j].x, s2);
+            s2 = fmaf(v[j].y, n[j].y, s2);
+            s2 = fmaf(v[j].z, n[j].z, s2);
+            s2 = fmaf(v[j].w, n[j].w, s2);
         }
         s1 = a.layer ? row_sum<G>(s1, slots[0]) * inv_d : 0.f;
         s2 = row_sum<G>(s2, slots[1]) * inv_d;
 #pragma unroll
         for (int j = 0; j < NCH; ++j) {
-            v[j] = (v[j] - s1 - n[j] * s2) * r + gs[j];
-            store_group(grad_h + row * D, 4 * (lane + G * j), D, v[j]);
+            v[j] = fma4(n[j], zero4 - s2, v[j] - s1) * r;
+            if (g_sum) v[j] += widen(gs[j]);
+            store_group<FULL>(grad_h + row * D, 4 * (lane + G * j), D, v[j]);
         }
         if (grad_branch) {
-            if (a.branch.kept < 65536u) drop_row<G>(v, k0, static_cast<unsigned>(row), lane, a.branch);
+            if (a.branch.kept < 65536u)
+                row_draws<G, NCH>(k0, static_cast<unsigned>(row), lane, [&](int j, unsigned lo, unsigned hi) {
+                    v[j] = drop_group(v[j], lo, hi, a.branch);
+                });
 #pragma unroll
-            for (int j = 0; j < NCH; ++j) store_group(grad_branch + row * D, 4 * (lane + G * j), D, v[j]);
+            for (int j = 0; j < NCH; ++j) store_group<FULL>(grad_branch + row * D, 4 * (lane + G * j), D, v[j]);
         }
         if constexpr (G > 64) __syncthreads();   // the next row's sums reuse the slots
     }
     if (!part) return;
     float* p = part + static_cast<size_t>(blockIdx.x) * 2 * D;
-    if constexpr (ROWS > 1) {   // the waves' sums, in fixed order
+#pragma unroll
+    for (int j = 0; j < NCH; ++j) {
+        gw[j] *= a.out.scale;
+        gb[j] *= a.out.scale;
+    }
+    if constexpr (ROWS > 1) {   // the sums of the workgroup's rows, in fixed order
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
 #pragma unroll
-            for (int j = 0; j < NCH; ++j) sums[threadIdx.x / G][lane + G * j] = half ? gb[j] : gw[j];
+            for (int j = 0; j < NCH; ++j) sums[at.sub][lane + G * j] = half ? gb[j] : gw[j];
             __syncthreads();
-            for (int q = threadIdx.x; 4 * q < D; q += WG) {
+            for (unsigned q = threadIdx.x; 4 * q < D; q += Place<G>::WG) {
                 f32x4 t = sums[0][q];
 #pragma unroll
                 for (int i = 1; i < ROWS; ++i) t += sums[i][q];
@@ -190,38 +224,50 @@ __global__ __launch_bounds__(1024) void norm_param_reduce_kernel(const float* __
     else static_cast<_Float16*>(to)[col] = static_cast<_Float16>(acc);
 }
 
-// How many workgroups share the rows; each leaves 2 D floats of sums.
-int slices_of(int64_t N, int64_t D) {
-    const int64_t rows = D <= 1024 ? 4 : 1, wgs = (N + rows - 1) / rows, most = D <= 1024 ? 768 : 512;
-    return static_cast<int>(wgs < most ? wgs : most);
+// How many workgroups share the rows at most; each leaves 2 D floats of sums.
+int64_t slices_of(int64_t N, int64_t D) {
+    const int64_t rows = D <= 128 ? 16 : D <= 1024 ? 4 : 1;
+    return workgroups(N, rows, D <= 4096 ? 4 * CUS : 2 * CUS);
 }
 
+template <class TO, class TH, class TB, int G, int NCH, bool FULL>
+int64_t go(const void* g, const void* g_sum, const void* h, const BackArgs& a, void* grad_h, void* grad_branch, float* part,
+           hipStream_t s) {
+    constexpr auto kernel = norm_backward_kernel<TO, TH, TB, G, NCH, FULL>;
+    constexpr int threads = Place<G>::WG;
+    static const int64_t most = CUS * resident(kernel, threads);
+    const int64_t slices = slices_of(a.N, a.D), wgs = slices <= most ? slices : workgroups(a.N, Place<G>::ROWS, most);
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(wgs)), dim3(threads), 0, s, static_cast<const TO*>(g),
+                       static_cast<const TH*>(g_sum), static_cast<const TH*>(h), a, static_cast<TH*>(grad_h),
+                       static_cast<TB*>(grad_branch), part);
+    return wgs;
+}
+
+// Returns how many slices of parameter sums there are in part (none without part).
 template <class TO, class TH, class TB>
-void launch_back(const void* g, const void* g_sum, const void* h, const BackArgs& a, void* grad_h, void* grad_branch,
-                 bool params, float* part, int slices, hipStream_t s) {
-    const TO* gp = static_cast<const TO*>(g);
-    const TH *gsp = static_cast<const TH*>(g_sum), *hp = static_cast<const TH*>(h);
-    TH* ghp = static_cast<TH*>(grad_h);
-    TB* gbp = static_cast<TB*>(grad_branch);
-    const dim3 grid(slices);
-#define T5VQ_NBK(G, NCH)                                                                                                  \
-    hipLaunchKernelGGL((norm_backward_kernel<TO, TH, TB, G, NCH>), grid, dim3(G > 256 ? G : 256), 0, s, gp, gsp, hp, a,   \
-                       ghp, gbp, params ? part : nullptr)
-    if (a.D <= 256) T5VQ_NBK(64, 1);
-    else if (a.D <= 512) T5VQ_NBK(64, 2);
-    else if (a.D <= 768) T5VQ_NBK(64, 3);
-    else if (a.D <= 1024) T5VQ_NBK(64, 4);
-    else if (a.D <= 2048) T5VQ_NBK(256, 2);
-    else if (a.D <= 4096) T5VQ_NBK(256, 4);
-    else if (a.D <= 8192) T5VQ_NBK(1024, 2);
-    else {
-        hipLaunchKernelGGL((norm_backward_rows_kernel<TO, TH, TB>), dim3(static_cast<unsigned>(a.N < 2048 ? a.N : 2048)),
-                           dim3(256), 0, s, gp, gsp, hp, a, ghp, gbp);
-        if (params)
-            hipLaunchKernelGGL((norm_param_grad_kernel<TO, TH>), dim3((a.D + 1023) / 1024, slices), dim3(256), 0, s, gp, hp, a,
-                               part);
-    }
+int64_t launch_back(const void* g, const void* g_sum, const void* h, const BackArgs& a, void* grad_h, void* grad_branch,
+                    float* part, hipStream_t s) {
+#define T5VQ_NBK(G, NCH)                                                                                       \
+    (a.D == 4 * G * NCH ? go<TO, TH, TB, G, NCH, true>(g, g_sum, h, a, grad_h, grad_branch, part, s)           \
+                        : go<TO, TH, TB, G, NCH, false>(g, g_sum, h, a, grad_h, grad_branch, part, s))
+    if (a.D <= 64) return T5VQ_NBK(16, 1);
+    if (a.D <= 128) return T5VQ_NBK(16, 2);
+    if (a.D <= 256) return T5VQ_NBK(64, 1);
+    if (a.D <= 512) return T5VQ_NBK(64, 2);
+    if (a.D <= 768) return T5VQ_NBK(64, 3);
+    if (a.D <= 1024) return T5VQ_NBK(64, 4);
+    if (a.D <= 2048) return T5VQ_NBK(256, 2);
+    if (a.D <= 4096) return T5VQ_NBK(256, 4);
+    if (a.D <= 8192) return T5VQ_NBK(1024, 2);
 #undef T5VQ_NBK
+    hipLaunchKernelGGL((norm_backward_rows_kernel<TO, TH, TB>), dim3(static_cast<unsigned>(workgroups(a.N, 1, CUS * 8))),
+                       dim3(256), 0, s, static_cast<const TO*>(g), static_cast<const TH*>(g_sum), static_cast<const TH*>(h), a,
+                       static_cast<TH*>(grad_h), static_cast<TB*>(grad_branch));
+    if (!part) return 0;
+    const int64_t slices = slices_of(a.N, a.D);
+    hipLaunchKernelGGL((norm_param_grad_kernel<TO, TH>), dim3((a.D + 1023) / 1024, static_cast<unsigned>(slices)), dim3(256), 0,
+                       s, static_cast<const TO*>(g), static_cast<const TH*>(h), a, part);
+    return slices;
 }
 
 }  // namespace
@@ -229,7 +275,7 @@ void launch_back(const void* g, const void* g_sum, const void* h, const BackArgs
 extern "C" {
 
 int64_t t5vq_norm_backward_workspace_bytes(int64_t N, int64_t D) {
-    return N > 0 && D > 0 ? static_cast<int64_t>(slices_of(N, D)) * 2 * D * 4 : 0;
+    return N > 0 && D > 0 ? slices_of(N, D) * 2 * D * 4 : 0;
 }
 
 int t5vq_norm_backward(const void* grad_out, int out_type, const void* grad_sum, const void* h, int hidden_type,
@@ -264,10 +310,10 @@ int t5vq_norm_backward(const void* grad_out, int out_type, const void* grad_sum,
     a.ctr = {0, 0, reinterpret_cast<const long long*>(ticket), ticket ? reinterpret_cast<const long long*>(ticket) + 1 : nullptr,
              nullptr};
     a.stats = stats;
-    float* part = static_cast<float*>(workspace);
-    const int slices = slices_of(N, D);
+    float* part = params ? static_cast<float*>(workspace) : nullptr;
+    int64_t slices = 0;
     hipStream_t s = static_cast<hipStream_t>(stream);
-#define T5VQ_NB(O, H, B) launch_back<O, H, B>(grad_out, grad_sum, h, a, grad_hidden, grad_branch, params, part, slices, s)
+#define T5VQ_NB(O, H, B) slices = launch_back<O, H, B>(grad_out, grad_sum, h, a, grad_hidden, grad_branch, part, s)
     if (hidden_type == T5VQ_BF16) out_type == T5VQ_F32 ? T5VQ_NB(float, __bf16, __bf16) : T5VQ_NB(__bf16, __bf16, __bf16);
     else if (hidden_type == T5VQ_F16)
         out_type == T5VQ_F32 ? T5VQ_NB(float, _Float16, _Float16) : T5VQ_NB(_Float16, _Float16, _Float16);
@@ -278,7 +324,7 @@ int t5vq_norm_backward(const void* grad_out, int out_type, const void* grad_sum,
     T5VQ_I_CHECK_HIP(hipGetLastError());
     if (params) {
         hipLaunchKernelGGL(norm_param_reduce_kernel, dim3(static_cast<unsigned>((D + 15) / 16), 2), dim3(1024), 0, s, part,
-                           slices, a.D, grad_weight, grad_bias, weight_type);
+                           static_cast<int>(slices), a.D, grad_weight, grad_bias, weight_type);
         T5VQ_I_CHECK_HIP(hipGetLastError());
     }
     return T5VQ_OK;
