@@ -51,11 +51,57 @@ __device__ __forceinline__ void store_group(T* __restrict__ row, unsigned c, uns
         if (c + 2 < D) row[c + 2] = static_cast<T>(v.z);
     }
 }
+// chunk j of a row whose chunks below SURE are whole (j known when unrolled)
+template <int SURE, class T>
+__device__ __forceinline__ void store_at(int j, T* __restrict__ row, unsigned c, unsigned D, f32x4 v) {
+    j < SURE ? store_group<true>(row, c, D, v) : store_group<false>(row, c, D, v);
+}
+template <int SURE, class T>
+__device__ __forceinline__ typename Group<T>::type load_at(int j, const T* __restrict__ row, unsigned c, unsigned D) {
+    return j < SURE ? load_raw<true>(row, c, D) : load_raw<false>(row, c, D);
+}
 template <class T>
 __device__ __forceinline__ f32x4 round_group(f32x4 v) {   // what a later read of the stored values gives
     typedef T V __attribute__((ext_vector_type(4)));
     return __builtin_convertvector(__builtin_convertvector(v, V), f32x4);
 }
+// eight elements: a Philox block's columns
+template <class T> struct Octet;
+template <> struct Octet<float> { typedef float type __attribute__((ext_vector_type(8), aligned(4))); };
+template <> struct Octet<__bf16> { typedef __bf16 type __attribute__((ext_vector_type(8), aligned(2))); };
+template <> struct Octet<_Float16> { typedef _Float16 type __attribute__((ext_vector_type(8), aligned(2))); };
+template <class T>
+__device__ __forceinline__ typename Octet<T>::type load_octet(const T* __restrict__ row, unsigned c, unsigned D) {
+    if (c + 8 <= D) return *reinterpret_cast<const typename Octet<T>::type*>(row + c);
+    const auto lo = load_raw<false>(row, c, D), hi = load_raw<false>(row, c + 4, D);
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+template <class V>
+__device__ __forceinline__ f32x4 low_half(V v) {
+    return __builtin_convertvector(__builtin_shufflevector(v, v, 0, 1, 2, 3), f32x4);
+}
+template <class V>
+__device__ __forceinline__ f32x4 high_half(V v) {
+    return __builtin_convertvector(__builtin_shufflevector(v, v, 4, 5, 6, 7), f32x4);
+}
+
+// floor(n / d) of any 32-bit n by a multiplication (Granlund, Montgomery: "Division by invariant integers using
+// multiplication", PLDI 1994, figure 4.1): with l = ceil(log2 d), m = floor(2^32 (2^l - d) / d) + 1 and t = high(m n) the
+// quotient is (t + ((n - t) >> min(l, 1))) >> max(l - 1, 0).
+struct Quotient {
+    unsigned d, m, s1, s2;
+    __device__ __forceinline__ unsigned of(unsigned n) const {
+        const unsigned t = __umulhi(m, n);
+        return (t + ((n - t) >> s1)) >> s2;
+    }
+};
+inline Quotient quotient_by(unsigned d) {
+    int l = 0;
+    while ((1ull << l) < d) ++l;
+    const unsigned m = static_cast<unsigned>((((1ull << l) - d) << 32) / d + 1);
+    return {d, m, l ? 1u : 0u, l ? static_cast<unsigned>(l - 1) : 0u};
+}
+
 // a parameter vector whose type is only known at run time (its reads are few: once per row at most, from cache)
 __device__ __forceinline__ f32x4 load_param(const void* p, int type, unsigned c, unsigned D) {
     if (type == T5VQ_F32) return load_group(static_cast<const float*>(p), c, D);
@@ -188,26 +234,30 @@ __device__ __forceinline__ void row_draws(Key k, unsigned row, unsigned lane, F 
     }
 }
 
-// where a thread stands: G lanes a row, a workgroup of at least 256 threads.  With a row to every wave or more the row is the
-// wave's, and kept in scalar registers.
-template <int G>
+// Where a thread stands: G lanes a row, WG threads a workgroup.  With a row to every wave or more the row is the wave's, and
+// kept in scalar registers.
+template <int G, int WG>
 struct Place {
-    static constexpr int WG = G > 256 ? G : 256, ROWS = WG / G;
+    static constexpr int ROWS = WG / G;
     unsigned lane, sub;
     __device__ __forceinline__ Place() {
-        lane = threadIdx.x & (G - 1);
+        lane = threadIdx.x % G;
         sub = threadIdx.x / G;
         if constexpr (G >= 64) sub = __builtin_amdgcn_readfirstlane(sub);
     }
 };
+// Chunks that are whole in every row a kernel of G lanes and NCH chunks is called for (launch_norm, launch_back): all of them
+// where D = 4 G NCH (FULL), all but the last else -- but for four chunks of 256 lanes or more, which start at half.
+template <int G, int NCH, bool FULL>
+constexpr int sure() { return FULL ? NCH : NCH == 4 && G >= 256 ? 2 : NCH - 1; }
 
-// sum over the G lanes of a row (16, or a multiple of 64), fixed order; slots: G / 64 floats of LDS, and one more set for the
-// next call, which may then write before every wave has read this one's
+// sum over the G lanes of a row (16, or a multiple of 64), fixed order; slots: G / 64 floats of LDS a row, and one more set for
+// the next call, which may then write before every wave has read this one's
 template <int G>
-__device__ __forceinline__ float row_sum(float v, float* slots) {
+__device__ __forceinline__ float row_sum(float v, float* slots, unsigned lane) {
     v = lanes_sum<(G < 64 ? G : 64)>(v);
     if constexpr (G > 64) {
-        if ((threadIdx.x & 63) == 0) slots[threadIdx.x >> 6] = v;
+        if ((lane & 63) == 0) slots[lane >> 6] = v;
         __syncthreads();
         v = 0.f;
 #pragma unroll

@@ -10,30 +10,58 @@ using namespace t5vq_norm;
 
 namespace {
 
-// y = residual + (kept ? x * scale : 0): one thread per block of eight columns, so each Philox block is drawn once.
-template <class TX, class TY, bool RES>
-__global__ __launch_bounds__(256) void dropout_add_kernel(const TX* __restrict__ x, const TY* __restrict__ res, int D,
-                                                          long long blocks, int per_row, Drop drop, Counter ctr,
+// y = residual + (kept ? x * scale : 0).  A thread takes U blocks of eight columns, 256 blocks apart, so that each Philox block
+// is drawn once and U blocks of every input are on their way together.  WHOLE: D % 8 == 0, rows follow each other without
+// a gap and a block is one access of 16 (half types) or two (fp32).
+template <class TX, class TY, bool RES, bool WHOLE>
+__global__ __launch_bounds__(256) void dropout_add_kernel(const TX* __restrict__ x, const TY* __restrict__ res, unsigned D,
+                                                          unsigned blocks, Quotient per_row, Drop drop, Counter ctr,
                                                           TY* __restrict__ y) {
+    constexpr int U = 2;
     if (ctr.ticket_out && blockIdx.x == 0 && threadIdx.x == 0) give_ticket(ctr);
-    const long long b = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
-    if (b >= blocks) return;
-    const long long row = b / per_row;
-    const int blk = static_cast<int>(b - row * per_row), c = blk * 8;
-    const TX* xr = x + row * D;
-    f32x4 lo = load_group(xr, c, D), hi = load_group(xr, c + 4, D);
-    if (drop.kept < 65536u) {
-        const Words w = philox(site_key(ctr, 0), blk, static_cast<unsigned>(row));
-        lo = drop_group(lo, w.w0, w.w1, drop);
-        hi = drop_group(hi, w.w2, w.w3, drop);
+    const unsigned first = blockIdx.x * (256u * U) + threadIdx.x;
+    typename Octet<TX>::type xv[U];
+    typename Octet<TY>::type rv[U];
+    unsigned row[U], blk[U];
+    size_t at[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const unsigned b = first + 256 * u;
+        if (b >= blocks) break;
+        row[u] = per_row.of(b);
+        blk[u] = b - row[u] * per_row.d;
+        at[u] = WHOLE ? static_cast<size_t>(b) * 8 : static_cast<size_t>(row[u]) * D;
+        if constexpr (WHOLE) {
+            xv[u] = *reinterpret_cast<const typename Octet<TX>::type*>(x + at[u]);
+            if constexpr (RES) rv[u] = *reinterpret_cast<const typename Octet<TY>::type*>(res + at[u]);
+        } else {
+            xv[u] = load_octet(x + at[u], blk[u] * 8, D);
+            if constexpr (RES) rv[u] = load_octet(res + at[u], blk[u] * 8, D);
+        }
     }
-    if constexpr (RES) {
-        const TY* rr = res + row * D;
-        lo = load_group(rr, c, D) + lo;
-        hi = load_group(rr, c + 4, D) + hi;
+    const Key key = site_key(ctr, 0);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        if (first + 256 * u >= blocks) break;
+        f32x4 lo = low_half(xv[u]), hi = high_half(xv[u]);
+        if (drop.kept < 65536u) {
+            const Words w = philox(key, blk[u], row[u]);
+            lo = drop_group(lo, w.w0, w.w1, drop);
+            hi = drop_group(hi, w.w2, w.w3, drop);
+        }
+        if constexpr (RES) {
+            lo = low_half(rv[u]) + lo;
+            hi = high_half(rv[u]) + hi;
+        }
+        if constexpr (WHOLE) {
+            typedef typename Octet<TY>::type V;
+            *reinterpret_cast<V*>(y + at[u]) =
+                __builtin_convertvector(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), V);
+        } else {
+            store_group(y + at[u], blk[u] * 8, D, lo);
+            store_group(y + at[u], blk[u] * 8 + 4, D, hi);
+        }
     }
-    store_group(y + row * D, c, D, lo);
-    store_group(y + row * D, c + 4, D, hi);
 }
 
 struct NormArgs {
@@ -53,12 +81,12 @@ struct NormArgs {
 // output; G = 16 (four rows a wave) or 64 (one) without a barrier, a workgroup a row above.  The parameters stay in registers
 // while a wave walks its rows, and the next row is on its way while this one is worked on.  FULL: D = 4 G NCH.
 template <class TH, class TB, class TO, bool ADD, int G, int NCH, bool FULL>
-__global__ __launch_bounds__(Place<G>::WG) void norm_kernel(const TH* __restrict__ hidden, const TB* __restrict__ branch,
+__global__ __launch_bounds__(G > 256 ? G : 256) void norm_kernel(const TH* __restrict__ hidden, const TB* __restrict__ branch,
                                                             TO* __restrict__ out, TH* __restrict__ sum, NormArgs a) {
-    constexpr int ROWS = Place<G>::ROWS;
+    constexpr int WG = G > 256 ? G : 256, ROWS = WG / G, SURE = sure<G, NCH, FULL>();
     __shared__ float slots[2][G > 64 ? G / 64 : 1];
     __shared__ f32x4 copy[std::is_same<TO, float>::value && G == 256 && NCH == 2 ? G * NCH : 1];
-    const Place<G> at;
+    const Place<G, WG> at;
     const unsigned lane = at.lane, D = FULL ? 4 * G * NCH : a.D;
     if (a.ctr.ticket_out && blockIdx.x == 0 && threadIdx.x == 0) give_ticket(a.ctr);
     const Key k0 = site_key(a.ctr, 0), k1 = site_key(a.ctr, 1);
@@ -77,8 +105,8 @@ __global__ __launch_bounds__(Place<G>::WG) void norm_kernel(const TH* __restrict
     auto fetch = [&](long long r) {
 #pragma unroll
         for (int j = 0; j < NCH; ++j) {
-            hn[j] = load_raw<FULL>(hidden + r * D, 4 * (lane + G * j), D);
-            if constexpr (ADD) bn[j] = load_raw<FULL>(branch + r * D, 4 * (lane + G * j), D);
+            hn[j] = load_at<SURE>(j, hidden + r * D, 4 * (lane + G * j), D);
+            if constexpr (ADD) bn[j] = load_at<SURE>(j, branch + r * D, 4 * (lane + G * j), D);
         }
     };
     if (row < a.N) fetch(row);
@@ -98,22 +126,22 @@ __global__ __launch_bounds__(Place<G>::WG) void norm_kernel(const TH* __restrict
 #pragma unroll
             for (int j = 0; j < NCH; ++j) {
                 h[j] = round_group<TH>(h[j] + br[j]);
-                store_group<FULL>(sum + row * D, 4 * (lane + G * j), D, h[j]);
+                store_at<SURE>(j, sum + row * D, 4 * (lane + G * j), D, h[j]);
             }
         }
         float mean = 0.f, s = 0.f;
         if (a.layer) {
 #pragma unroll
             for (int j = 0; j < NCH; ++j) s = sum4(h[j], s);
-            mean = row_sum<G>(s, slots[0]) * inv_d;
+            mean = row_sum<G>(s, slots[0], lane) * inv_d;
             s = 0.f;
         }
 #pragma unroll
         for (int j = 0; j < NCH; ++j) {
-            h[j] = inside<FULL>(h[j] - mean, 4 * (lane + G * j), D);
+            h[j] = j < SURE ? h[j] - mean : inside<false>(h[j] - mean, 4 * (lane + G * j), D);
             s = sq4(h[j], s);
         }
-        const float r = 1.0f / __fsqrt_rn(row_sum<G>(s, slots[1]) * inv_d + a.eps);
+        const float r = 1.0f / __fsqrt_rn(row_sum<G>(s, slots[1], lane) * inv_d + a.eps);
         if (a.stats && lane == 0) {
             a.stats[2 * row] = mean;
             a.stats[2 * row + 1] = r;
@@ -125,7 +153,7 @@ __global__ __launch_bounds__(Place<G>::WG) void norm_kernel(const TH* __restrict
                 h[j] = keep_group(h[j], lo, hi, a.out.kept);
             });
 #pragma unroll
-        for (int j = 0; j < NCH; ++j) store_group<FULL>(out + row * D, 4 * (lane + G * j), D, h[j]);
+        for (int j = 0; j < NCH; ++j) store_at<SURE>(j, out + row * D, 4 * (lane + G * j), D, h[j]);
         if constexpr (std::is_same<TO, float>::value && 4 * G * NCH <= 2048) {   // what the searches take of fp32 rows
             if (a.xx || a.img.rows) {
                 float m = 0.f, inv;
@@ -227,9 +255,9 @@ __global__ __launch_bounds__(256) void norm_rows_kernel(const TH* __restrict__ h
 template <class TH, class TB, class TO, bool ADD, int G, int NCH, bool FULL>
 void go(const void* hidden, const void* branch, void* out, void* sum, const NormArgs& a, hipStream_t stream) {
     constexpr auto kernel = norm_kernel<TH, TB, TO, ADD, G, NCH, FULL>;
-    constexpr int threads = Place<G>::WG;
+    constexpr int threads = G > 256 ? G : 256;
     static const int64_t most = CUS * resident(kernel, threads);
-    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(workgroups(a.N, Place<G>::ROWS, most))), dim3(threads), 0, stream,
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(workgroups(a.N, threads / G, most))), dim3(threads), 0, stream,
                        static_cast<const TH*>(hidden), static_cast<const TB*>(branch), static_cast<TO*>(out),
                        static_cast<TH*>(sum), a);
 }
@@ -260,15 +288,19 @@ template <class TX, class TY>
 void launch_dropout(const void* x, const void* res, void* y, int64_t N, int64_t D, Drop drop, const Counter& ctr,
                     hipStream_t stream) {
     const int64_t per_row = (D + 7) / 8, blocks = N * per_row;
-    const dim3 grid(static_cast<unsigned>((blocks + 255) / 256));
-    if (res)
-        hipLaunchKernelGGL((dropout_add_kernel<TX, TY, true>), grid, dim3(256), 0, stream, static_cast<const TX*>(x),
-                           static_cast<const TY*>(res), static_cast<int>(D), blocks, static_cast<int>(per_row), drop, ctr,
-                           static_cast<TY*>(y));
-    else
-        hipLaunchKernelGGL((dropout_add_kernel<TX, TY, false>), grid, dim3(256), 0, stream, static_cast<const TX*>(x),
-                           static_cast<const TY*>(res), static_cast<int>(D), blocks, static_cast<int>(per_row), drop, ctr,
-                           static_cast<TY*>(y));
+#define T5VQ_DK(RES, WHOLE)                                                                                          \
+    hipLaunchKernelGGL((dropout_add_kernel<TX, TY, RES, WHOLE>), dim3(static_cast<unsigned>((blocks + 511) / 512)), \
+                       dim3(256), 0, stream, static_cast<const TX*>(x), static_cast<const TY*>(res),                \
+                       static_cast<unsigned>(D), static_cast<unsigned>(blocks),                                      \
+                       quotient_by(static_cast<unsigned>(per_row)), drop, ctr, static_cast<TY*>(y))
+    if (D % 8 == 0) {
+        if (res) T5VQ_DK(true, true);
+        else T5VQ_DK(false, true);
+    } else {
+        if (res) T5VQ_DK(true, false);
+        else T5VQ_DK(false, false);
+    }
+#undef T5VQ_DK
 }
 
 }  // namespace
@@ -287,7 +319,7 @@ int t5vq_dropout_add(const void* x, int x_type, const void* residual, int64_t N,
     T5VQ_I_REQUIRE(known_type(x_type) && known_type(y_type), "unknown element type");
     T5VQ_I_REQUIRE(x_type == y_type || x_type == T5VQ_F32 || y_type == T5VQ_F32, "bf16 and f16 do not meet in one call");
     T5VQ_I_REQUIRE(N > 0 && N <= 0xFFFFFFFFLL && D > 0 && D <= (1LL << 30), "N, D out of range");
-    T5VQ_I_REQUIRE(N * ((D + 7) / 8) <= 0xFFFFFF00LL, "more than 2^35 elements in one launch");
+    T5VQ_I_REQUIRE(N * ((D + 7) / 8) <= 0xFFFFFE00LL, "more than 2^35 elements in one launch");
     T5VQ_I_REQUIRE(t5vq_dropout_keep_count(p) >= 0, "p must be in [0, 1]");
     T5VQ_I_REQUIRE(aligned_to(x, x_type) && aligned_to(y, y_type) && (!residual || aligned_to(residual, y_type)),
                    "elements must be aligned");

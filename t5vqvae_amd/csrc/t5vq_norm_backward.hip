@@ -29,15 +29,15 @@ __device__ __forceinline__ float block_sum(float v, float* slots) {   // 256 thr
 //   grad_weight = sum over rows of gy n, grad_bias = sum of gy.
 // The row stays in registers between its two sums and its gradients (group lane + G * j in chunk j, as forward), and a wave
 // adds up the parameters' gradients of all rows it walks: every input is read once.  Workgroup b leaves its sums in part[b].
-template <class TO, class TH, class TB, int G, int NCH, bool FULL>
-__global__ __launch_bounds__(Place<G>::WG) void norm_backward_kernel(const TO* __restrict__ g, const TH* __restrict__ g_sum,
+template <class TO, class TH, class TB, int G, int NCH, int WG, bool FULL>
+__global__ __launch_bounds__(WG) void norm_backward_kernel(const TO* __restrict__ g, const TH* __restrict__ g_sum,
                                                                      const TH* __restrict__ h, BackArgs a,
                                                                      TH* __restrict__ grad_h, TB* __restrict__ grad_branch,
                                                                      float* __restrict__ part) {
-    constexpr int ROWS = Place<G>::ROWS;
-    __shared__ float slots[2][G > 64 ? G / 64 : 1];
+    constexpr int ROWS = WG / G, SURE = sure<G, NCH, FULL>();
+    __shared__ float slots[2][G > 64 ? ROWS : 1][G > 64 ? G / 64 : 1];
     __shared__ f32x4 sums[ROWS > 1 ? ROWS : 1][ROWS > 1 ? G * NCH : 1];
-    const Place<G> at;
+    const Place<G, WG> at;
     const unsigned lane = at.lane, D = FULL ? 4 * G * NCH : a.D;
     const Key k0 = site_key(a.ctr, 0), k1 = site_key(a.ctr, 1);
     const f32x4 zero4 = {0.f, 0.f, 0.f, 0.f};
@@ -50,31 +50,35 @@ __global__ __launch_bounds__(Place<G>::WG) void norm_backward_kernel(const TO* _
     }
     const float inv_d = 1.0f / static_cast<float>(D);
     const long long step = static_cast<long long>(gridDim.x) * ROWS;
-    long long row = static_cast<long long>(blockIdx.x) * ROWS + at.sub;
+    const long long first = static_cast<long long>(blockIdx.x) * ROWS;
     typename Group<TO>::type vn[NCH];
     typename Group<TH>::type nn[NCH], sn[NCH];
     float mean_n = 0.f, r_n = 0.f;
     auto fetch = [&](long long t) {
 #pragma unroll
         for (int j = 0; j < NCH; ++j) {
-            vn[j] = load_raw<FULL>(g + t * D, 4 * (lane + G * j), D);
-            nn[j] = load_raw<FULL>(h + t * D, 4 * (lane + G * j), D);
+            vn[j] = load_at<SURE>(j, g + t * D, 4 * (lane + G * j), D);
+            nn[j] = load_at<SURE>(j, h + t * D, 4 * (lane + G * j), D);
         }
         if (g_sum) {
 #pragma unroll
-            for (int j = 0; j < NCH; ++j) sn[j] = load_raw<FULL>(g_sum + t * D, 4 * (lane + G * j), D);
+            for (int j = 0; j < NCH; ++j) sn[j] = load_at<SURE>(j, g_sum + t * D, 4 * (lane + G * j), D);
         }
         mean_n = a.stats[2 * t];
         r_n = a.stats[2 * t + 1];
     };
-    if (row < a.N) fetch(row);
-    for (; row < a.N; row += step) {
+    if (first + at.sub < a.N) fetch(first + at.sub);
+    for (long long base = first; base < a.N; base += step) {
+        const long long row = base + at.sub;
+        // where waves wait for each other every one of them comes along, with a row of its own or without
+        const bool live = row < a.N;
+        if (G <= 64 && !live) break;
         f32x4 v[NCH], n[NCH];
         typename Group<TH>::type gs[NCH];
 #pragma unroll
         for (int j = 0; j < NCH; ++j) {
-            v[j] = widen(vn[j]);
-            n[j] = widen(nn[j]);
+            v[j] = live ? widen(vn[j]) : zero4;
+            n[j] = live ? widen(nn[j]) : zero4;
             gs[j] = sn[j];
         }
         const float mean = mean_n, r = r_n;
@@ -96,21 +100,21 @@ __global__ __launch_bounds__(Place<G>::WG) void norm_backward_kernel(const TO* _
             s2 = fmaf(v[j].z, n[j].z, s2);
             s2 = fmaf(v[j].w, n[j].w, s2);
         }
-        s1 = a.layer ? row_sum<G>(s1, slots[0]) * inv_d : 0.f;
-        s2 = row_sum<G>(s2, slots[1]) * inv_d;
+        s1 = a.layer ? row_sum<G>(s1, slots[0][G > 64 ? at.sub : 0], lane) * inv_d : 0.f;
+        s2 = row_sum<G>(s2, slots[1][G > 64 ? at.sub : 0], lane) * inv_d;
 #pragma unroll
         for (int j = 0; j < NCH; ++j) {
             v[j] = fma4(n[j], zero4 - s2, v[j] - s1) * r;
             if (g_sum) v[j] += widen(gs[j]);
-            store_group<FULL>(grad_h + row * D, 4 * (lane + G * j), D, v[j]);
+            if (live) store_at<SURE>(j, grad_h + row * D, 4 * (lane + G * j), D, v[j]);
         }
-        if (grad_branch) {
+        if (grad_branch && live) {
             if (a.branch.kept < 65536u)
                 row_draws<G, NCH>(k0, static_cast<unsigned>(row), lane, [&](int j, unsigned lo, unsigned hi) {
                     v[j] = drop_group(v[j], lo, hi, a.branch);
                 });
 #pragma unroll
-            for (int j = 0; j < NCH; ++j) store_group<FULL>(grad_branch + row * D, 4 * (lane + G * j), D, v[j]);
+            for (int j = 0; j < NCH; ++j) store_at<SURE>(j, grad_branch + row * D, 4 * (lane + G * j), D, v[j]);
         }
         if constexpr (G > 64) __syncthreads();   // the next row's sums reuse the slots
     }
@@ -127,7 +131,7 @@ __global__ __launch_bounds__(Place<G>::WG) void norm_backward_kernel(const TO* _
 #pragma unroll
             for (int j = 0; j < NCH; ++j) sums[at.sub][lane + G * j] = half ? gb[j] : gw[j];
             __syncthreads();
-            for (unsigned q = threadIdx.x; 4 * q < D; q += Place<G>::WG) {
+            for (unsigned q = threadIdx.x; 4 * q < D; q += WG) {
                 f32x4 t = sums[0][q];
 #pragma unroll
                 for (int i = 1; i < ROWS; ++i) t += sums[i][q];
@@ -225,19 +229,15 @@ __global__ __launch_bounds__(1024) void norm_param_reduce_kernel(const float* __
 }
 
 // How many workgroups share the rows at most; each leaves 2 D floats of sums.
-int64_t slices_of(int64_t N, int64_t D) {
-    const int64_t rows = D <= 128 ? 16 : D <= 1024 ? 4 : 1;
-    return workgroups(N, rows, D <= 4096 ? 4 * CUS : 2 * CUS);
-}
+int64_t slices_of(int64_t N) { return N < 2 * CUS ? N : 2 * CUS; }
 
-template <class TO, class TH, class TB, int G, int NCH, bool FULL>
+template <class TO, class TH, class TB, int G, int NCH, int WG, bool FULL>
 int64_t go(const void* g, const void* g_sum, const void* h, const BackArgs& a, void* grad_h, void* grad_branch, float* part,
            hipStream_t s) {
-    constexpr auto kernel = norm_backward_kernel<TO, TH, TB, G, NCH, FULL>;
-    constexpr int threads = Place<G>::WG;
-    static const int64_t most = CUS * resident(kernel, threads);
-    const int64_t slices = slices_of(a.N, a.D), wgs = slices <= most ? slices : workgroups(a.N, Place<G>::ROWS, most);
-    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(wgs)), dim3(threads), 0, s, static_cast<const TO*>(g),
+    constexpr auto kernel = norm_backward_kernel<TO, TH, TB, G, NCH, WG, FULL>;
+    static const int64_t most = CUS * resident(kernel, WG);
+    const int64_t wgs = workgroups(a.N, WG / G, most < 2 * CUS ? most : 2 * CUS);
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(wgs)), dim3(WG), 0, s, static_cast<const TO*>(g),
                        static_cast<const TH*>(g_sum), static_cast<const TH*>(h), a, static_cast<TH*>(grad_h),
                        static_cast<TB*>(grad_branch), part);
     return wgs;
@@ -247,24 +247,24 @@ int64_t go(const void* g, const void* g_sum, const void* h, const BackArgs& a, v
 template <class TO, class TH, class TB>
 int64_t launch_back(const void* g, const void* g_sum, const void* h, const BackArgs& a, void* grad_h, void* grad_branch,
                     float* part, hipStream_t s) {
-#define T5VQ_NBK(G, NCH)                                                                                       \
-    (a.D == 4 * G * NCH ? go<TO, TH, TB, G, NCH, true>(g, g_sum, h, a, grad_h, grad_branch, part, s)           \
-                        : go<TO, TH, TB, G, NCH, false>(g, g_sum, h, a, grad_h, grad_branch, part, s))
-    if (a.D <= 64) return T5VQ_NBK(16, 1);
-    if (a.D <= 128) return T5VQ_NBK(16, 2);
-    if (a.D <= 256) return T5VQ_NBK(64, 1);
-    if (a.D <= 512) return T5VQ_NBK(64, 2);
-    if (a.D <= 768) return T5VQ_NBK(64, 3);
-    if (a.D <= 1024) return T5VQ_NBK(64, 4);
-    if (a.D <= 2048) return T5VQ_NBK(256, 2);
-    if (a.D <= 4096) return T5VQ_NBK(256, 4);
-    if (a.D <= 8192) return T5VQ_NBK(1024, 2);
+#define T5VQ_NBK(G, NCH, WG)                                                                                       \
+    (a.D == 4 * G * NCH ? go<TO, TH, TB, G, NCH, WG, true>(g, g_sum, h, a, grad_h, grad_branch, part, s)           \
+                        : go<TO, TH, TB, G, NCH, WG, false>(g, g_sum, h, a, grad_h, grad_branch, part, s))
+    if (a.D <= 64) return T5VQ_NBK(16, 1, 768);
+    if (a.D <= 128) return T5VQ_NBK(16, 2, 768);
+    if (a.D <= 256) return T5VQ_NBK(64, 1, 768);
+    if (a.D <= 512) return T5VQ_NBK(64, 2, 768);
+    if (a.D <= 768) return T5VQ_NBK(64, 3, 768);
+    if (a.D <= 1024) return T5VQ_NBK(64, 4, 512);
+    if (a.D <= 2048) return T5VQ_NBK(256, 2, 1024);
+    if (a.D <= 4096) return T5VQ_NBK(256, 4, 512);
+    if (a.D <= 8192) return T5VQ_NBK(1024, 2, 1024);
 #undef T5VQ_NBK
     hipLaunchKernelGGL((norm_backward_rows_kernel<TO, TH, TB>), dim3(static_cast<unsigned>(workgroups(a.N, 1, CUS * 8))),
                        dim3(256), 0, s, static_cast<const TO*>(g), static_cast<const TH*>(g_sum), static_cast<const TH*>(h), a,
                        static_cast<TH*>(grad_h), static_cast<TB*>(grad_branch));
     if (!part) return 0;
-    const int64_t slices = slices_of(a.N, a.D);
+    const int64_t slices = slices_of(a.N);
     hipLaunchKernelGGL((norm_param_grad_kernel<TO, TH>), dim3((a.D + 1023) / 1024, static_cast<unsigned>(slices)), dim3(256), 0,
                        s, static_cast<const TO*>(g), static_cast<const TH*>(h), a, part);
     return slices;
@@ -275,7 +275,7 @@ int64_t launch_back(const void* g, const void* g_sum, const void* h, const BackA
 extern "C" {
 
 int64_t t5vq_norm_backward_workspace_bytes(int64_t N, int64_t D) {
-    return N > 0 && D > 0 ? slices_of(N, D) * 2 * D * 4 : 0;
+    return N > 0 && D > 0 ? slices_of(N) * 2 * D * 4 : 0;
 }
 
 int t5vq_norm_backward(const void* grad_out, int out_type, const void* grad_sum, const void* h, int hidden_type,
