@@ -54,11 +54,28 @@ __device__ __forceinline__ void store_group(T* __restrict__ row, unsigned c, uns
 // chunk j of a row whose chunks below SURE are whole (j known when unrolled)
 template <int SURE, class T>
 __device__ __forceinline__ void store_at(int j, T* __restrict__ row, unsigned c, unsigned D, f32x4 v) {
-    j < SURE ? store_group<true>(row, c, D, v) : store_group<false>(row, c, D, v);
+    typedef typename Group<T>::type V;
+    if (j < SURE || c + 4 <= D)   // the row's pointer is the wave's, the lane's place 32 bits: one scalar base, one offset
+        *reinterpret_cast<V*>(reinterpret_cast<char*>(row) + c * static_cast<unsigned>(sizeof(T))) = __builtin_convertvector(v, V);
+    else
+        store_group<false>(row, c, D, v);
 }
+// Reads of the other chunks do not branch (a branch would wait for every read already on its way): a group that reaches past
+// the row's end, or lies behind it, reads the row's last four elements (D >= 4), and widen_at puts them in their places
+// when they are there, 0 behind the end.
 template <int SURE, class T>
 __device__ __forceinline__ typename Group<T>::type load_at(int j, const T* __restrict__ row, unsigned c, unsigned D) {
-    return j < SURE ? load_raw<true>(row, c, D) : load_raw<false>(row, c, D);
+    const unsigned at = (j < SURE || c + 4 <= D ? c : D - 4) * static_cast<unsigned>(sizeof(T));
+    return *reinterpret_cast<const typename Group<T>::type*>(reinterpret_cast<const char*>(row) + at);
+}
+template <int SURE, class V>
+__device__ __forceinline__ f32x4 widen_at(int j, V raw, unsigned c, unsigned D) {
+    const f32x4 v = widen(raw), zero = {0.f, 0.f, 0.f, 0.f};
+    if (j < SURE) return v;
+    const unsigned behind = (0u - D) & 3u;   // how many of the last group's columns do not exist: the same for the whole call
+    const f32x4 last = {behind == 1 ? v.y : behind == 2 ? v.z : v.w, behind == 1 ? v.z : behind == 2 ? v.w : 0.f,
+                        behind == 1 ? v.w : 0.f, 0.f};
+    return c + 4 <= D ? v : (c < D ? last : zero);
 }
 template <class T>
 __device__ __forceinline__ f32x4 round_group(f32x4 v) {   // what a later read of the stored values gives

@@ -114,8 +114,8 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void norm_kernel(const TH* __res
         f32x4 h[NCH], br[ADD ? NCH : 1];
 #pragma unroll
         for (int j = 0; j < NCH; ++j) {
-            h[j] = widen(hn[j]);
-            if constexpr (ADD) br[j] = widen(bn[j]);
+            h[j] = widen_at<SURE>(j, hn[j], 4 * (lane + G * j), D);
+            if constexpr (ADD) br[j] = widen_at<SURE>(j, bn[j], 4 * (lane + G * j), D);
         }
         if (row + step < a.N) fetch(row + step);
         if constexpr (ADD) {
@@ -203,7 +203,7 @@ __device__ __forceinline__ float block_sum(float v, float* slots) {   // 256 thr
     return (slots[0] + slots[1]) + (slots[2] + slots[3]);
 }
 
-// Rows that registers do not hold (D > 16384): one workgroup per row, read again from memory for each of its sums.
+// Rows that registers do not hold (D > 16384), and rows shorter than one group (D < 4): one workgroup per row, read again from memory for each of its sums.
 template <class TH, class TB, class TO, bool ADD>
 __global__ __launch_bounds__(256) void norm_rows_kernel(const TH* __restrict__ hidden, const TB* __restrict__ branch,
                                                         TO* __restrict__ out, TH* __restrict__ sum, NormArgs a) {
@@ -267,7 +267,11 @@ void launch_norm(const void* hidden, const void* branch, void* out, void* sum, c
 #define T5VQ_NK(G, NCH)                                                                                        \
     (a.D == 4 * G * NCH ? go<TH, TB, TO, ADD, G, NCH, true>(hidden, branch, out, sum, a, stream)               \
                         : go<TH, TB, TO, ADD, G, NCH, false>(hidden, branch, out, sum, a, stream))
-    if (a.D <= 64) T5VQ_NK(16, 1);
+    if (a.D < 4 || a.D > 16384)
+        hipLaunchKernelGGL((norm_rows_kernel<TH, TB, TO, ADD>), dim3(static_cast<unsigned>(workgroups(a.N, 1, CUS * 8))),
+                           dim3(256), 0, stream, static_cast<const TH*>(hidden), static_cast<const TB*>(branch),
+                           static_cast<TO*>(out), static_cast<TH*>(sum), a);
+    else if (a.D <= 64) T5VQ_NK(16, 1);
     else if (a.D <= 128) T5VQ_NK(16, 2);
     else if (a.D <= 256) T5VQ_NK(64, 1);
     else if (a.D <= 512) T5VQ_NK(64, 2);
@@ -276,11 +280,7 @@ void launch_norm(const void* hidden, const void* branch, void* out, void* sum, c
     else if (a.D <= 2048) T5VQ_NK(256, 2);
     else if (a.D <= 4096) T5VQ_NK(256, 4);
     else if (a.D <= 8192) T5VQ_NK(1024, 2);
-    else if (a.D <= 16384) T5VQ_NK(1024, 4);
-    else
-        hipLaunchKernelGGL((norm_rows_kernel<TH, TB, TO, ADD>), dim3(static_cast<unsigned>(workgroups(a.N, 1, CUS * 8))),
-                           dim3(256), 0, stream, static_cast<const TH*>(hidden), static_cast<const TB*>(branch),
-                           static_cast<TO*>(out), static_cast<TH*>(sum), a);
+    else T5VQ_NK(1024, 4);
 #undef T5VQ_NK
 }
 

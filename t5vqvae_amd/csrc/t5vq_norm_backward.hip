@@ -77,8 +77,8 @@ __global__ __launch_bounds__(WG) void norm_backward_kernel(const TO* __restrict_
         typename Group<TH>::type gs[NCH];
 #pragma unroll
         for (int j = 0; j < NCH; ++j) {
-            v[j] = live ? widen(vn[j]) : zero4;
-            n[j] = live ? widen(nn[j]) : zero4;
+            v[j] = live ? widen_at<SURE>(j, vn[j], 4 * (lane + G * j), D) : zero4;
+            n[j] = live ? widen_at<SURE>(j, nn[j], 4 * (lane + G * j), D) : zero4;
             gs[j] = sn[j];
         }
         const float mean = mean_n, r = r_n;
@@ -105,7 +105,7 @@ __global__ __launch_bounds__(WG) void norm_backward_kernel(const TO* __restrict_
 #pragma unroll
         for (int j = 0; j < NCH; ++j) {
             v[j] = fma4(n[j], zero4 - s2, v[j] - s1) * r;
-            if (g_sum) v[j] += widen(gs[j]);
+            if (g_sum) v[j] += widen_at<SURE>(j, gs[j], 4 * (lane + G * j), D);
             if (live) store_at<SURE>(j, grad_h + row * D, 4 * (lane + G * j), D, v[j]);
         }
         if (grad_branch && live) {
@@ -148,7 +148,7 @@ __global__ __launch_bounds__(WG) void norm_backward_kernel(const TO* __restrict_
     }
 }
 
-// Rows that registers do not hold (D > 8192): one workgroup per row, read once for its sums and once for its gradients.
+// Rows that registers do not hold (D > 8192), and rows shorter than one group (D < 4): one workgroup per row, read once for its sums and once for its gradients.
 template <class TO, class TH, class TB>
 __global__ __launch_bounds__(256) void norm_backward_rows_kernel(const TO* __restrict__ g, const TH* __restrict__ g_sum,
                                                                  const TH* __restrict__ h, BackArgs a,
@@ -247,18 +247,22 @@ int64_t go(const void* g, const void* g_sum, const void* h, const BackArgs& a, v
 template <class TO, class TH, class TB>
 int64_t launch_back(const void* g, const void* g_sum, const void* h, const BackArgs& a, void* grad_h, void* grad_branch,
                     float* part, hipStream_t s) {
-#define T5VQ_NBK(G, NCH, WG)                                                                                       \
-    (a.D == 4 * G * NCH ? go<TO, TH, TB, G, NCH, WG, true>(g, g_sum, h, a, grad_h, grad_branch, part, s)           \
+// WG, WG2: one workgroup fills a CU with the waves that its registers leave room for (occupancy 2 .. 4 of a SIMD's 512
+// registers), so that few workgroups leave sums behind; whole rows of the half types need the fewest registers.
+#define T5VQ_NBK(G, NCH, WG, WG2)                                                                                  \
+    (a.D == 4 * G * NCH ? go<TO, TH, TB, G, NCH, sizeof(TH) == 2 ? WG2 : WG, true>(g, g_sum, h, a, grad_h, grad_branch, part, s) \
                         : go<TO, TH, TB, G, NCH, WG, false>(g, g_sum, h, a, grad_h, grad_branch, part, s))
-    if (a.D <= 64) return T5VQ_NBK(16, 1, 768);
-    if (a.D <= 128) return T5VQ_NBK(16, 2, 768);
-    if (a.D <= 256) return T5VQ_NBK(64, 1, 768);
-    if (a.D <= 512) return T5VQ_NBK(64, 2, 768);
-    if (a.D <= 768) return T5VQ_NBK(64, 3, 768);
-    if (a.D <= 1024) return T5VQ_NBK(64, 4, 512);
-    if (a.D <= 2048) return T5VQ_NBK(256, 2, 1024);
-    if (a.D <= 4096) return T5VQ_NBK(256, 4, 512);
-    if (a.D <= 8192) return T5VQ_NBK(1024, 2, 1024);
+    if (a.D >= 4 && a.D <= 8192) {
+        if (a.D <= 64) return T5VQ_NBK(16, 1, 768, 768);
+        if (a.D <= 128) return T5VQ_NBK(16, 2, 768, 768);
+        if (a.D <= 256) return T5VQ_NBK(64, 1, 768, 768);
+        if (a.D <= 512) return T5VQ_NBK(64, 2, 768, 768);
+        if (a.D <= 768) return T5VQ_NBK(64, 3, 768, 1024);
+        if (a.D <= 1024) return T5VQ_NBK(64, 4, 512, 768);
+        if (a.D <= 2048) return T5VQ_NBK(256, 2, 1024, 1024);
+        if (a.D <= 4096) return T5VQ_NBK(256, 4, 512, 768);
+        return T5VQ_NBK(1024, 2, 1024, 1024);
+    }
 #undef T5VQ_NBK
     hipLaunchKernelGGL((norm_backward_rows_kernel<TO, TH, TB>), dim3(static_cast<unsigned>(workgroups(a.N, 1, CUS * 8))),
                        dim3(256), 0, s, static_cast<const TO*>(g), static_cast<const TH*>(g_sum), static_cast<const TH*>(h), a,
