@@ -19,6 +19,12 @@ template <> struct Group<float> { typedef float type __attribute__((ext_vector_t
 template <> struct Group<__bf16> { typedef __bf16 type __attribute__((ext_vector_type(4), aligned(2))); };
 template <> struct Group<_Float16> { typedef _Float16 type __attribute__((ext_vector_type(4), aligned(2))); };
 
+// eight elements: a Philox block's columns
+template <class T> struct Octet;
+template <> struct Octet<float> { typedef float type __attribute__((ext_vector_type(8), aligned(4))); };
+template <> struct Octet<__bf16> { typedef __bf16 type __attribute__((ext_vector_type(8), aligned(2))); };
+template <> struct Octet<_Float16> { typedef _Float16 type __attribute__((ext_vector_type(8), aligned(2))); };
+
 // Columns c .. c + 3 of a row of D elements, as they are in memory; columns >= D read as 0.  FULL: there are none (a row that
 // fills every lane's groups: no comparison, no branch).
 template <bool FULL, class T>
@@ -77,31 +83,21 @@ __device__ __forceinline__ f32x4 widen_at(int j, V raw, unsigned c, unsigned D) 
                         behind == 1 ? v.w : 0.f, 0.f};
     return c + 4 <= D ? v : (c < D ? last : zero);
 }
+// a block's two groups, read as load_at reads them, and one of them widened (FROM: 0 or 4)
+template <class T>
+__device__ __forceinline__ typename Octet<T>::type load_octet(const T* __restrict__ row, unsigned c, unsigned D) {
+    const auto lo = load_at<0>(0, row, c, D), hi = load_at<0>(0, row, c + 4, D);
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+template <int SURE, int FROM, class V>
+__device__ __forceinline__ f32x4 half_at(V v, unsigned c, unsigned D) {
+    return widen_at<SURE>(0, __builtin_shufflevector(v, v, FROM, FROM + 1, FROM + 2, FROM + 3), c, D);
+}
 template <class T>
 __device__ __forceinline__ f32x4 round_group(f32x4 v) {   // what a later read of the stored values gives
     typedef T V __attribute__((ext_vector_type(4)));
     return __builtin_convertvector(__builtin_convertvector(v, V), f32x4);
 }
-// eight elements: a Philox block's columns
-template <class T> struct Octet;
-template <> struct Octet<float> { typedef float type __attribute__((ext_vector_type(8), aligned(4))); };
-template <> struct Octet<__bf16> { typedef __bf16 type __attribute__((ext_vector_type(8), aligned(2))); };
-template <> struct Octet<_Float16> { typedef _Float16 type __attribute__((ext_vector_type(8), aligned(2))); };
-template <class T>
-__device__ __forceinline__ typename Octet<T>::type load_octet(const T* __restrict__ row, unsigned c, unsigned D) {
-    if (c + 8 <= D) return *reinterpret_cast<const typename Octet<T>::type*>(row + c);
-    const auto lo = load_raw<false>(row, c, D), hi = load_raw<false>(row, c + 4, D);
-    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-}
-template <class V>
-__device__ __forceinline__ f32x4 low_half(V v) {
-    return __builtin_convertvector(__builtin_shufflevector(v, v, 0, 1, 2, 3), f32x4);
-}
-template <class V>
-__device__ __forceinline__ f32x4 high_half(V v) {
-    return __builtin_convertvector(__builtin_shufflevector(v, v, 4, 5, 6, 7), f32x4);
-}
-
 // floor(n / d) of any 32-bit n by a multiplication (Granlund, Montgomery: "Division by invariant integers using
 // multiplication", PLDI 1994, figure 4.1): with l = ceil(log2 d), m = floor(2^32 (2^l - d) / d) + 1 and t = high(m n) the
 // quotient is (t + ((n - t) >> min(l, 1))) >> max(l - 1, 0).

@@ -35,7 +35,7 @@ __global__ __launch_bounds__(256) void dropout_add_kernel(const TX* __restrict__
             xv[u] = *reinterpret_cast<const typename Octet<TX>::type*>(x + at[u]);
             if constexpr (RES) rv[u] = *reinterpret_cast<const typename Octet<TY>::type*>(res + at[u]);
         } else {
-            xv[u] = load_octet(x + at[u], blk[u] * 8, D);
+            xv[u] = load_octet(x + at[u], blk[u] * 8, D);     // D >= 4, see load_at
             if constexpr (RES) rv[u] = load_octet(res + at[u], blk[u] * 8, D);
         }
     }
@@ -43,25 +43,40 @@ __global__ __launch_bounds__(256) void dropout_add_kernel(const TX* __restrict__
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         if (first + 256 * u >= blocks) break;
-        f32x4 lo = low_half(xv[u]), hi = high_half(xv[u]);
+        const unsigned c = blk[u] * 8;
+        constexpr int SURE = WHOLE ? 1 : 0;
+        f32x4 lo = half_at<SURE, 0>(xv[u], c, D), hi = half_at<SURE, 4>(xv[u], c + 4, D);
         if (drop.kept < 65536u) {
             const Words w = philox(key, blk[u], row[u]);
             lo = drop_group(lo, w.w0, w.w1, drop);
             hi = drop_group(hi, w.w2, w.w3, drop);
         }
         if constexpr (RES) {
-            lo = low_half(rv[u]) + lo;
-            hi = high_half(rv[u]) + hi;
+            lo = half_at<SURE, 0>(rv[u], c, D) + lo;
+            hi = half_at<SURE, 4>(rv[u], c + 4, D) + hi;
         }
         if constexpr (WHOLE) {
             typedef typename Octet<TY>::type V;
             *reinterpret_cast<V*>(y + at[u]) =
                 __builtin_convertvector(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), V);
         } else {
-            store_group(y + at[u], blk[u] * 8, D, lo);
-            store_group(y + at[u], blk[u] * 8 + 4, D, hi);
+            store_group(y + at[u], c, D, lo);
+            store_group(y + at[u], c + 4, D, hi);
         }
     }
+}
+
+// rows of one to three columns: a thread each
+template <class TX, class TY>
+__global__ __launch_bounds__(256) void dropout_add_short_kernel(const TX* __restrict__ x, const TY* __restrict__ res, unsigned D,
+                                                                long long N, Drop drop, Counter ctr, TY* __restrict__ y) {
+    const long long row = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+    if (ctr.ticket_out && row == 0) give_ticket(ctr);
+    if (row >= N) return;
+    f32x4 v = load_group(x + row * D, 0, D);
+    if (drop.kept < 65536u) v = drop_at(v, site_key(ctr, 0), 0, static_cast<unsigned>(row), drop);
+    if (res) v = load_group(res + row * D, 0, D) + v;
+    store_group(y + row * D, 0, D, v);
 }
 
 struct NormArgs {
@@ -293,7 +308,11 @@ void launch_dropout(const void* x, const void* res, void* y, int64_t N, int64_t 
                        dim3(256), 0, stream, static_cast<const TX*>(x), static_cast<const TY*>(res),                \
                        static_cast<unsigned>(D), static_cast<unsigned>(blocks),                                      \
                        quotient_by(static_cast<unsigned>(per_row)), drop, ctr, static_cast<TY*>(y))
-    if (D % 8 == 0) {
+    if (D < 4) {
+        hipLaunchKernelGGL((dropout_add_short_kernel<TX, TY>), dim3(static_cast<unsigned>((N + 255) / 256)), dim3(256), 0, stream,
+                           static_cast<const TX*>(x), static_cast<const TY*>(res), static_cast<unsigned>(D), N, drop, ctr,
+                           static_cast<TY*>(y));
+    } else if (D % 8 == 0) {
         if (res) T5VQ_DK(true, true);
         else T5VQ_DK(false, true);
     } else {
