@@ -122,6 +122,14 @@ __device__ __forceinline__ f32x4 load_param(const void* p, int type, unsigned c,
     return load_group(static_cast<const _Float16*>(p), c, D);
 }
 
+// a parameter's gradient, in the parameter's type; p may be null
+__device__ __forceinline__ void store_param(void* p, int type, unsigned c, unsigned D, f32x4 v) {
+    if (!p) return;
+    if (type == T5VQ_F32) store_group(static_cast<float*>(p), c, D, v);
+    else if (type == T5VQ_BF16) store_group(static_cast<__bf16*>(p), c, D, v);
+    else store_group(static_cast<_Float16*>(p), c, D, v);
+}
+
 // ---- random numbers -------------------------------------------------------------------------------------------------
 // Where a call's random numbers come from (host side): seed / offset by value, or read from device memory on top (a
 // generator under graph capture, or a ticket).
@@ -226,25 +234,39 @@ __device__ __forceinline__ f32x4 fma4(const f32x4 a, const f32x4 b, const f32x4 
 __device__ __forceinline__ float sum4(const f32x4 v, float s) { return s + ((v.x + v.y) + (v.z + v.w)); }
 
 // Draws for a row held in registers, group lane + G * j in chunk j (G even).  Neighbouring lanes hold the two halves of a
-// block; for two chunks j, j + 1 the even lane draws chunk j's block and the odd lane chunk j + 1's, and each hands its
-// neighbour the two words it needs: half the draws of every lane drawing for itself.  f(j, lo, hi) gets chunk j's bits.
+// block, so of two draws that both lanes need, the even lane makes one and the odd lane the other, and each hands its
+// neighbour the two words it needs: half the draws of every lane drawing for itself.
+struct Bits { unsigned lo, hi; };   // of one group
+__device__ __forceinline__ void share(const Words w, bool odd, Bits& evens, Bits& odds) {
+    const unsigned r0 = __builtin_amdgcn_mov_dpp(odd ? w.w0 : w.w2, 0xB1, 0xF, 0xF, true);   // quad_perm [1, 0, 3, 2]
+    const unsigned r1 = __builtin_amdgcn_mov_dpp(odd ? w.w1 : w.w3, 0xB1, 0xF, 0xF, true);
+    evens = odd ? Bits{r0, r1} : Bits{w.w0, w.w1};
+    odds = odd ? Bits{w.w2, w.w3} : Bits{r0, r1};
+}
+// f(j, bits of chunk j) for all chunks but the last of an odd number: pairs of chunks share
 template <int G, int NCH, class F>
-__device__ __forceinline__ void row_draws(Key k, unsigned row, unsigned lane, F f) {
+__device__ __forceinline__ void pair_draws(Key k, unsigned row, unsigned lane, F f) {
     const bool odd = lane & 1;
 #pragma unroll
     for (int j = 0; j + 1 < NCH; j += 2) {
-        const Words w = philox(k, ((lane >> 1) + (G / 2) * j) + (odd ? G / 2 : 0), row);
-        const unsigned s0 = odd ? w.w0 : w.w2, s1 = odd ? w.w1 : w.w3;      // the neighbour's half of my block
-        const unsigned m0 = odd ? w.w2 : w.w0, m1 = odd ? w.w3 : w.w1;      // mine
-        const unsigned r0 = __builtin_amdgcn_mov_dpp(s0, 0xB1, 0xF, 0xF, true);   // quad_perm [1, 0, 3, 2]
-        const unsigned r1 = __builtin_amdgcn_mov_dpp(s1, 0xB1, 0xF, 0xF, true);
-        f(j, odd ? r0 : m0, odd ? r1 : m1);
-        f(j + 1, odd ? m0 : r0, odd ? m1 : r1);
+        Bits b0, b1;
+        share(philox(k, ((lane >> 1) + (G / 2) * j) + (odd ? G / 2 : 0), row), odd, b0, b1);
+        f(j, b0);
+        f(j + 1, b1);
     }
-    if constexpr (NCH & 1) {
-        const Words w = philox(k, (lane >> 1) + (G / 2) * (NCH - 1), row);
-        f(NCH - 1, odd ? w.w2 : w.w0, odd ? w.w3 : w.w1);
-    }
+}
+// bits of the last of an odd number of chunks: two sites of a row share (evens: of k0, odds: of k1) ...
+template <int G, int NCH>
+__device__ __forceinline__ void last_draws(Key k0, Key k1, unsigned row, unsigned lane, Bits& b0, Bits& b1) {
+    const bool odd = lane & 1;
+    const Key k = {k0.k0, k0.k1, odd ? k1.c0 : k0.c0, odd ? k1.c1 : k0.c1};
+    share(philox(k, (lane >> 1) + (G / 2) * (NCH - 1), row), odd, b0, b1);
+}
+// ... or, where one site draws, this row and the one that the lane walks next
+template <int G, int NCH>
+__device__ __forceinline__ void last_draws(Key k, unsigned row, unsigned next, unsigned lane, Bits& now, Bits& then) {
+    const bool odd = lane & 1;
+    share(philox(k, (lane >> 1) + (G / 2) * (NCH - 1), odd ? next : row), odd, now, then);
 }
 
 // Where a thread stands: G lanes a row, WG threads a workgroup.  With a row to every wave or more the row is the wave's, and

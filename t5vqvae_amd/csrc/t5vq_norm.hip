@@ -124,8 +124,12 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void norm_kernel(const TH* __res
             if constexpr (ADD) bn[j] = load_at<SURE>(j, branch + r * D, 4 * (lane + G * j), D);
         }
     };
+    const bool drops = ADD && a.branch.kept < 65536u, drops_out = a.out.kept < 65536u;
+    Bits last0 = {0, 0}, last1 = {0, 0};   // of the last of an odd number of chunks, where a draw gave it in advance
+    bool ahead = false;
     if (row < a.N) fetch(row);
     for (; row < a.N; row += step) {
+        const unsigned r32 = static_cast<unsigned>(row);
         f32x4 h[NCH], br[ADD ? NCH : 1];
 #pragma unroll
         for (int j = 0; j < NCH; ++j) {
@@ -133,11 +137,22 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void norm_kernel(const TH* __res
             if constexpr (ADD) br[j] = widen_at<SURE>(j, bn[j], 4 * (lane + G * j), D);
         }
         if (row + step < a.N) fetch(row + step);
+        Bits bits = {0, 0};
+        if constexpr (NCH & 1) {
+            if (drops && drops_out) {
+                last_draws<G, NCH>(k0, k1, r32, lane, last0, bits);
+            } else if (drops || drops_out) {
+                if (!ahead) last_draws<G, NCH>(drops ? k0 : k1, r32, static_cast<unsigned>(row + step), lane, bits, last1);
+                else bits = last1;
+                ahead = !ahead;
+                last0 = bits;
+            }
+        }
         if constexpr (ADD) {
-            if (a.branch.kept < 65536u)
-                row_draws<G, NCH>(k0, static_cast<unsigned>(row), lane, [&](int j, unsigned lo, unsigned hi) {
-                    br[j] = drop_group(br[j], lo, hi, a.branch);
-                });
+            if (drops) {
+                pair_draws<G, NCH>(k0, r32, lane, [&](int j, Bits b) { br[j] = drop_group(br[j], b.lo, b.hi, a.branch); });
+                if constexpr (NCH & 1) br[NCH - 1] = drop_group(br[NCH - 1], last0.lo, last0.hi, a.branch);
+            }
 #pragma unroll
             for (int j = 0; j < NCH; ++j) {
                 h[j] = round_group<TH>(h[j] + br[j]);
@@ -163,10 +178,10 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void norm_kernel(const TH* __res
         }
 #pragma unroll
         for (int j = 0; j < NCH; ++j) h[j] = fma4(h[j] * r, w[j], b[j]);
-        if (a.out.kept < 65536u)
-            row_draws<G, NCH>(k1, static_cast<unsigned>(row), lane, [&](int j, unsigned lo, unsigned hi) {
-                h[j] = keep_group(h[j], lo, hi, a.out.kept);
-            });
+        if (drops_out) {
+            pair_draws<G, NCH>(k1, r32, lane, [&](int j, Bits b) { h[j] = keep_group(h[j], b.lo, b.hi, a.out.kept); });
+            if constexpr (NCH & 1) h[NCH - 1] = keep_group(h[NCH - 1], bits.lo, bits.hi, a.out.kept);
+        }
 #pragma unroll
         for (int j = 0; j < NCH; ++j) store_at<SURE>(j, out + row * D, 4 * (lane + G * j), D, h[j]);
         if constexpr (std::is_same<TO, float>::value && 4 * G * NCH <= 2048) {   // what the searches take of fp32 rows

@@ -14,6 +14,7 @@ struct BackArgs {
     Drop branch, out;
     Counter ctr;
     const float* stats;   // [N, 2]
+    void *grad_weight, *grad_bias;
 };
 
 __device__ __forceinline__ float block_sum(float v, float* slots) {   // 256 threads; fixed order
@@ -67,6 +68,9 @@ __global__ __launch_bounds__(WG) void norm_backward_kernel(const TO* __restrict_
         mean_n = a.stats[2 * t];
         r_n = a.stats[2 * t + 1];
     };
+    const bool drops = grad_branch && a.branch.kept < 65536u, drops_out = a.out.kept < 65536u;
+    Bits last0 = {0, 0}, last1 = {0, 0};   // of the last of an odd number of chunks, where a draw gave it in advance
+    bool ahead = false;
     if (first + at.sub < a.N) fetch(first + at.sub);
     for (long long base = first; base < a.N; base += step) {
         const long long row = base + at.sub;
@@ -83,10 +87,22 @@ __global__ __launch_bounds__(WG) void norm_backward_kernel(const TO* __restrict_
         }
         const float mean = mean_n, r = r_n;
         if (row + step < a.N) fetch(row + step);
-        if (a.out.kept < 65536u)
-            row_draws<G, NCH>(k1, static_cast<unsigned>(row), lane, [&](int j, unsigned lo, unsigned hi) {
-                v[j] = keep_group(v[j], lo, hi, a.out.kept);
-            });
+        const unsigned r32 = static_cast<unsigned>(row);
+        Bits bits = {0, 0};
+        if constexpr (NCH & 1) {
+            if (drops && drops_out) {
+                last_draws<G, NCH>(k0, k1, r32, lane, last0, bits);
+            } else if (drops || drops_out) {
+                if (!ahead) last_draws<G, NCH>(drops ? k0 : k1, r32, static_cast<unsigned>(row + step), lane, bits, last1);
+                else bits = last1;
+                ahead = !ahead;
+                last0 = bits;
+            }
+        }
+        if (drops_out) {
+            pair_draws<G, NCH>(k1, r32, lane, [&](int j, Bits b) { v[j] = keep_group(v[j], b.lo, b.hi, a.out.kept); });
+            if constexpr (NCH & 1) v[NCH - 1] = keep_group(v[NCH - 1], bits.lo, bits.hi, a.out.kept);
+        }
         float s1 = 0.f, s2 = 0.f;
 #pragma unroll
         for (int j = 0; j < NCH; ++j) {
@@ -109,10 +125,10 @@ __global__ __launch_bounds__(WG) void norm_backward_kernel(const TO* __restrict_
             if (live) store_at<SURE>(j, grad_h + row * D, 4 * (lane + G * j), D, v[j]);
         }
         if (grad_branch && live) {
-            if (a.branch.kept < 65536u)
-                row_draws<G, NCH>(k0, static_cast<unsigned>(row), lane, [&](int j, unsigned lo, unsigned hi) {
-                    v[j] = drop_group(v[j], lo, hi, a.branch);
-                });
+            if (drops) {
+                pair_draws<G, NCH>(k0, r32, lane, [&](int j, Bits b) { v[j] = drop_group(v[j], b.lo, b.hi, a.branch); });
+                if constexpr (NCH & 1) v[NCH - 1] = drop_group(v[NCH - 1], last0.lo, last0.hi, a.branch);
+            }
 #pragma unroll
             for (int j = 0; j < NCH; ++j) store_at<SURE>(j, grad_branch + row * D, 4 * (lane + G * j), D, v[j]);
         }
@@ -120,6 +136,7 @@ __global__ __launch_bounds__(WG) void norm_backward_kernel(const TO* __restrict_
     }
     if (!part) return;
     float* p = part + static_cast<size_t>(blockIdx.x) * 2 * D;
+    const bool only = gridDim.x == 1;   // no other workgroup's sums to add: these are the gradients
 #pragma unroll
     for (int j = 0; j < NCH; ++j) {
         gw[j] *= a.out.scale;
@@ -135,15 +152,21 @@ __global__ __launch_bounds__(WG) void norm_backward_kernel(const TO* __restrict_
                 f32x4 t = sums[0][q];
 #pragma unroll
                 for (int i = 1; i < ROWS; ++i) t += sums[i][q];
-                store_group(p + half * D, 4 * q, D, t);
+                if (only) store_param(half ? a.grad_bias : a.grad_weight, a.weight_type, 4 * q, D, t);
+                else store_group(p + half * D, 4 * q, D, t);
             }
             __syncthreads();
         }
     } else {
 #pragma unroll
         for (int j = 0; j < NCH; ++j) {
-            store_group(p, 4 * (lane + G * j), D, gw[j]);
-            store_group(p + D, 4 * (lane + G * j), D, gb[j]);
+            if (only) {
+                store_param(a.grad_weight, a.weight_type, 4 * (lane + G * j), D, gw[j]);
+                store_param(a.grad_bias, a.weight_type, 4 * (lane + G * j), D, gb[j]);
+            } else {
+                store_group(p, 4 * (lane + G * j), D, gw[j]);
+                store_group(p + D, 4 * (lane + G * j), D, gb[j]);
+            }
         }
     }
 }
@@ -236,14 +259,15 @@ int64_t go(const void* g, const void* g_sum, const void* h, const BackArgs& a, v
            hipStream_t s) {
     constexpr auto kernel = norm_backward_kernel<TO, TH, TB, G, NCH, WG, FULL>;
     static const int64_t most = CUS * resident(kernel, WG);
-    const int64_t wgs = workgroups(a.N, WG / G, most < 2 * CUS ? most : 2 * CUS);
+    // up to four rows a wave one workgroup takes them all: its turns cost less than a second launch
+    const int64_t wgs = a.N <= 4 * (WG / G) && part ? 1 : workgroups(a.N, WG / G, most < 2 * CUS ? most : 2 * CUS);
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(wgs)), dim3(WG), 0, s, static_cast<const TO*>(g),
                        static_cast<const TH*>(g_sum), static_cast<const TH*>(h), a, static_cast<TH*>(grad_h),
                        static_cast<TB*>(grad_branch), part);
-    return wgs;
+    return wgs > 1 ? wgs : 0;
 }
 
-// Returns how many slices of parameter sums there are in part (none without part).
+// Returns how many slices of parameter sums there are in part to be added (0: the gradients are written already).
 template <class TO, class TH, class TB>
 int64_t launch_back(const void* g, const void* g_sum, const void* h, const BackArgs& a, void* grad_h, void* grad_branch,
                     float* part, hipStream_t s) {
@@ -313,7 +337,7 @@ int t5vq_norm_backward(const void* grad_out, int out_type, const void* grad_sum,
     a.branch = make_drop(branch_p), a.out = make_drop(p);
     a.ctr = {0, 0, reinterpret_cast<const long long*>(ticket), ticket ? reinterpret_cast<const long long*>(ticket) + 1 : nullptr,
              nullptr};
-    a.stats = stats;
+    a.stats = stats, a.grad_weight = grad_weight, a.grad_bias = grad_bias;
     float* part = params ? static_cast<float*>(workspace) : nullptr;
     int64_t slices = 0;
     hipStream_t s = static_cast<hipStream_t>(stream);
@@ -326,7 +350,7 @@ int t5vq_norm_backward(const void* grad_out, int out_type, const void* grad_sum,
     else T5VQ_NB(float, float, _Float16);
 #undef T5VQ_NB
     T5VQ_I_CHECK_HIP(hipGetLastError());
-    if (params) {
+    if (params && slices) {
         hipLaunchKernelGGL(norm_param_reduce_kernel, dim3(static_cast<unsigned>((D + 15) / 16), 2), dim3(1024), 0, s, part,
                            static_cast<int>(slices), a.D, grad_weight, grad_bias, weight_type);
         T5VQ_I_CHECK_HIP(hipGetLastError());
