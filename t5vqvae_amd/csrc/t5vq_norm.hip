@@ -189,12 +189,14 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void norm_kernel(const TH* __res
                 float m = 0.f, inv;
                 s = 0.f;
                 if constexpr (G <= 64) {
+                    // 16 lanes: chunk j is what lanes 16 j .. 16 j + 15 of a wave hold, added by its steps of 32 and 16
+                    float q[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int j = 0; j < NCH; ++j) {
-                        // 16 lanes: the groups of a second chunk belong to a wave's lanes 16 .. 31, a chain of their own
-                        s = G < 64 ? s + sq4(h[j], 0.f) : sq4(h[j], s);
+                        q[G < 64 ? j : 0] = sq4(h[j], q[G < 64 ? j : 0]);
                         m = t5vq_absmax4(m, h[j].x, h[j].y, h[j].z, h[j].w);
                     }
+                    s = G < 64 ? (q[0] + q[2]) + (q[1] + q[3]) : q[0];
                 } else {   // a row's norm is defined on one wave's lanes: through LDS, every wave adds all of it
 #pragma unroll
                     for (int j = 0; j < NCH; ++j) copy[lane + G * j] = h[j];
@@ -303,7 +305,8 @@ void launch_norm(const void* hidden, const void* branch, void* out, void* sum, c
                            static_cast<TO*>(out), static_cast<TH*>(sum), a);
     else if (a.D <= 64) T5VQ_NK(16, 1);
     else if (a.D <= 128) T5VQ_NK(16, 2);
-    else if (a.D <= 256) T5VQ_NK(64, 1);
+    else if (a.D <= 192) T5VQ_NK(16, 3);
+    else if (a.D <= 256) T5VQ_NK(16, 4);
     else if (a.D <= 512) T5VQ_NK(64, 2);
     else if (a.D <= 768) T5VQ_NK(64, 3);
     else if (a.D <= 1024) T5VQ_NK(64, 4);

@@ -279,7 +279,8 @@ int64_t launch_back(const void* g, const void* g_sum, const void* h, const BackA
     if (a.D >= 4 && a.D <= 8192) {
         if (a.D <= 64) return T5VQ_NBK(16, 1, 768, 768);
         if (a.D <= 128) return T5VQ_NBK(16, 2, 768, 768);
-        if (a.D <= 256) return T5VQ_NBK(64, 1, 768, 768);
+        if (a.D <= 192) return T5VQ_NBK(16, 3, 768, 768);
+        if (a.D <= 256) return T5VQ_NBK(16, 4, 512, 512);
         if (a.D <= 512) return T5VQ_NBK(64, 2, 768, 768);
         if (a.D <= 768) return T5VQ_NBK(64, 3, 768, 1024);
         if (a.D <= 1024) return T5VQ_NBK(64, 4, 512, 768);
