@@ -1,4 +1,5 @@
-// Internal to libt5vq.so: what the dropout / norm kernels share (t5vq_norm.hip, t5vq_norm_backward.hip).
+// Internal to libt5vq.so: what the dropout / norm kernels share (t5vq_norm.hip: dropout and the C ABI;
+// t5vq_norm_f32 / _bf16 / _f16.hip: the norms of one type of rows, from t5vq_norm_forward.h and t5vq_norm_backward.h).
 //
 // Rows are walked in GROUPS of four consecutive columns: group q = columns 4q .. 4q + 3, one group per lane.  A row of any
 // length starts at any multiple of its element's size, so group accesses promise the compiler no more than the element's
@@ -57,22 +58,27 @@ __device__ __forceinline__ void store_group(T* __restrict__ row, unsigned c, uns
         if (c + 2 < D) row[c + 2] = static_cast<T>(v.z);
     }
 }
-// chunk j of a row whose chunks below SURE are whole (j known when unrolled)
-template <int SURE, class T>
+// chunk j of a row whose chunks below SURE are whole (j known when unrolled); STREAM: past the caches
+template <int SURE, bool STREAM = false, class T>
 __device__ __forceinline__ void store_at(int j, T* __restrict__ row, unsigned c, unsigned D, f32x4 v) {
     typedef typename Group<T>::type V;
-    if (j < SURE || c + 4 <= D)   // the row's pointer is the wave's, the lane's place 32 bits: one scalar base, one offset
-        *reinterpret_cast<V*>(reinterpret_cast<char*>(row) + c * static_cast<unsigned>(sizeof(T))) = __builtin_convertvector(v, V);
-    else
+    if (j < SURE || c + 4 <= D) {   // the row's pointer is the wave's, the lane's place 32 bits: one scalar base, one offset
+        V* p = reinterpret_cast<V*>(reinterpret_cast<char*>(row) + c * static_cast<unsigned>(sizeof(T)));
+        if constexpr (STREAM) __builtin_nontemporal_store(__builtin_convertvector(v, V), p);
+        else *p = __builtin_convertvector(v, V);
+    } else {
         store_group<false>(row, c, D, v);
+    }
 }
 // Reads of the other chunks do not branch (a branch would wait for every read already on its way): a group that reaches past
 // the row's end, or lies behind it, reads the row's last four elements (D >= 4), and widen_at puts them in their places
 // when they are there, 0 behind the end.
-template <int SURE, class T>
+template <int SURE, bool STREAM = false, class T>
 __device__ __forceinline__ typename Group<T>::type load_at(int j, const T* __restrict__ row, unsigned c, unsigned D) {
     const unsigned at = (j < SURE || c + 4 <= D ? c : D - 4) * static_cast<unsigned>(sizeof(T));
-    return *reinterpret_cast<const typename Group<T>::type*>(reinterpret_cast<const char*>(row) + at);
+    const auto* p = reinterpret_cast<const typename Group<T>::type*>(reinterpret_cast<const char*>(row) + at);
+    if constexpr (STREAM) return __builtin_nontemporal_load(p);
+    else return *p;
 }
 template <int SURE, class V>
 __device__ __forceinline__ f32x4 widen_at(int j, V raw, unsigned c, unsigned D) {
@@ -269,6 +275,14 @@ __device__ __forceinline__ void last_draws(Key k, unsigned row, unsigned next, u
     share(philox(k, (lane >> 1) + (G / 2) * (NCH - 1), odd ? next : row), odd, now, then);
 }
 
+// What a row kernel knows of its rows: that they fill their chunks exactly (WHOLE), and then that a call moves so much that
+// the caches keep nothing of it (STREAMED: reads and writes go past them).
+enum { RAGGED, WHOLE, STREAMED };
+// From 1.5 times the 256 MB of the last cache: 65536 x 768 fp32 rms norm 77 -> 73 us, its backward 124 -> 117 us, add + norm
+// 155 -> 145 us and backward 206 -> 194 us; below, what a neighbouring kernel left there is lost (16384 x 768 fp32 norm
+// 17 -> 21 us, 65536 x 768 bf16 backward, 300 MB, 61 -> 66 us).
+constexpr int64_t STREAM_BYTES = 384ll << 20;
+
 // Where a thread stands: G lanes a row, WG threads a workgroup.  With a row to every wave or more the row is the wave's, and
 // kept in scalar registers.
 template <int G, int WG>
@@ -282,9 +296,9 @@ struct Place {
     }
 };
 // Chunks that are whole in every row a kernel of G lanes and NCH chunks is called for (launch_norm, launch_back): all of them
-// where D = 4 G NCH (FULL), all but the last else -- but for four chunks of 256 lanes or more, which start at half.
-template <int G, int NCH, bool FULL>
-constexpr int sure() { return FULL ? NCH : NCH == 4 && G >= 256 ? 2 : NCH - 1; }
+// where D = 4 G NCH, all but the last else -- but for four chunks of 256 lanes or more, which start at half.
+template <int G, int NCH, int MODE>
+constexpr int sure() { return MODE != RAGGED ? NCH : NCH == 4 && G >= 256 ? 2 : NCH - 1; }
 
 // sum over the G lanes of a row (16, or a multiple of 64), fixed order; slots: G / 64 floats of LDS a row, and one more set for
 // the next call, which may then write before every wave has read this one's
@@ -299,6 +313,13 @@ __device__ __forceinline__ float row_sum(float v, float* slots, unsigned lane) {
         for (int i = 0; i < G / 64; ++i) v += slots[i];
     }
     return v;
+}
+__device__ __forceinline__ float block_sum(float v, float* slots) {   // 256 threads; fixed order
+    v = wave_sum(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) slots[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return (slots[0] + slots[1]) + (slots[2] + slots[3]);
 }
 // values of columns >= D to 0 (they only exist in a row's last group and behind it)
 template <bool FULL>
@@ -327,6 +348,43 @@ inline int64_t workgroups(int64_t N, int64_t rows, int64_t most) {
     const int64_t turns = (wgs + most - 1) / most;
     return (wgs + turns - 1) / turns;
 }
+
+struct NormArgs {
+    const void* weight;
+    const void* bias;
+    int weight_type, layer, D;
+    long long N;
+    float eps;
+    Drop branch, out;
+    Counter ctr;
+    float* stats;     // [N, 2]: mean (0 for rms), 1 / sqrt(variance + eps)
+    float* xx;        // [N]
+    T5vqTokenImage img;
+};
+
+struct BackArgs {
+    const void* weight;
+    int weight_type, layer, D;
+    long long N;
+    Drop branch, out;
+    Counter ctr;
+    const float* stats;   // [N, 2]
+    void *grad_weight, *grad_bias;
+};
+
+// The norms of rows of one type (hidden); part: the parameters' sums or null; backward returns how many slices of them are
+// left to be added (0: the gradients are written already).
+#define T5VQ_NORM_TYPED(NAME)                                                                                              \
+    void forward_##NAME(const void* hidden, const void* branch, int branch_type, void* out, int out_type, void* sum,       \
+                        const NormArgs& a, hipStream_t stream);                                                            \
+    int64_t backward_##NAME(const void* g, int out_type, const void* g_sum, const void* h, const BackArgs& a, void* grad_h, \
+                            void* grad_branch, int branch_type, float* part, hipStream_t stream);
+T5VQ_NORM_TYPED(f32)
+T5VQ_NORM_TYPED(bf16)
+T5VQ_NORM_TYPED(f16)
+#undef T5VQ_NORM_TYPED
+// How many workgroups share the rows of a backward call at most; each leaves 2 D floats of sums.
+inline int64_t slices_of(int64_t N) { return N < 2 * CUS ? N : 2 * CUS; }
 
 inline bool known_type(int t) { return t == T5VQ_F32 || t == T5VQ_BF16 || t == T5VQ_F16; }
 inline int64_t type_bytes(int t) { return t == T5VQ_F32 ? 4 : 2; }

@@ -1,9 +1,7 @@
-// t5vq_norm.hip -- dropout from a counter, and the norms of an encoder with that dropout: forward.  gfx950 kernels + C ABI;
-// include/t5vq.h has the contract.  Backward: t5vq_norm_backward.hip.
+// t5vq_norm.hip -- dropout from a counter (gfx950 kernels), and the C ABI of dropout and the norms; include/t5vq.h has the
+// contract.  The norms' own kernels: t5vq_norm_forward.h, t5vq_norm_backward.h.
 //
 // Compiled with -ffp-contract=off: every fused multiply-add below is an explicit fmaf().
-#include <type_traits>
-
 #include "t5vq_norm.h"
 
 using namespace t5vq_norm;
@@ -79,242 +77,29 @@ __global__ __launch_bounds__(256) void dropout_add_short_kernel(const TX* __rest
     store_group(y + row * D, 0, D, v);
 }
 
-struct NormArgs {
-    const void* weight;
-    const void* bias;
-    int weight_type, layer, D;
-    long long N;
-    float eps;
-    Drop branch, out;
-    Counter ctr;
-    float* stats;     // [N, 2]: mean (0 for rms), 1 / sqrt(variance + eps)
-    float* xx;        // [N]
-    T5vqTokenImage img;
-};
-
-// A row in registers: G lanes hold it, group lane + G * j in chunk j of NCH.  One read of each input, one write of each
-// output; G = 16 (four rows a wave) or 64 (one) without a barrier, a workgroup a row above.  The parameters stay in registers
-// while a wave walks its rows, and the next row is on its way while this one is worked on.  FULL: D = 4 G NCH.
-template <class TH, class TB, class TO, bool ADD, int G, int NCH, bool FULL>
-__global__ __launch_bounds__(G > 256 ? G : 256) void norm_kernel(const TH* __restrict__ hidden, const TB* __restrict__ branch,
-                                                            TO* __restrict__ out, TH* __restrict__ sum, NormArgs a) {
-    constexpr int WG = G > 256 ? G : 256, ROWS = WG / G, SURE = sure<G, NCH, FULL>();
-    __shared__ float slots[2][G > 64 ? G / 64 : 1];
-    __shared__ f32x4 copy[std::is_same<TO, float>::value && G == 256 && NCH == 2 ? G * NCH : 1];
-    const Place<G, WG> at;
-    const unsigned lane = at.lane, D = FULL ? 4 * G * NCH : a.D;
-    if (a.ctr.ticket_out && blockIdx.x == 0 && threadIdx.x == 0) give_ticket(a.ctr);
-    const Key k0 = site_key(a.ctr, 0), k1 = site_key(a.ctr, 1);
-    const f32x4 zero4 = {0.f, 0.f, 0.f, 0.f};
-    f32x4 w[NCH], b[NCH];           // times the output's scale: a kept value needs no multiplication of its own
+// part[slices][2][D] to the two gradients: 16 columns x 64 slice groups a workgroup, one tree over the groups -- a fixed order
+__global__ __launch_bounds__(1024) void norm_param_reduce_kernel(const float* __restrict__ part, int slices, int D,
+                                                                 void* __restrict__ grad_weight,
+                                                                 void* __restrict__ grad_bias, int type) {
+    __shared__ float sums[64][17];
+    const int c = threadIdx.x & 15, s0 = threadIdx.x >> 4, col = blockIdx.x * 16 + c;
+    void* to = blockIdx.y ? grad_bias : grad_weight;
+    if (!to) return;
+    const float* p = part + static_cast<size_t>(blockIdx.y) * D + col;
+    float acc = 0.f;
+    if (col < D)
+        for (int s = s0; s < slices; s += 64) acc += p[static_cast<size_t>(s) * 2 * D];
+    sums[s0][c] = acc;
 #pragma unroll
-    for (int j = 0; j < NCH; ++j) {
-        w[j] = load_param(a.weight, a.weight_type, 4 * (lane + G * j), D) * a.out.scale;
-        b[j] = a.bias ? load_param(a.bias, a.weight_type, 4 * (lane + G * j), D) * a.out.scale : zero4;
+    for (int o = 32; o > 0; o >>= 1) {
+        __syncthreads();
+        if (s0 < o) sums[s0][c] += sums[s0 + o][c];
     }
-    const float inv_d = 1.0f / static_cast<float>(D);
-    const long long step = static_cast<long long>(gridDim.x) * ROWS;
-    long long row = static_cast<long long>(blockIdx.x) * ROWS + at.sub;
-    typename Group<TH>::type hn[NCH];
-    typename Group<TB>::type bn[NCH];
-    auto fetch = [&](long long r) {
-#pragma unroll
-        for (int j = 0; j < NCH; ++j) {
-            hn[j] = load_at<SURE>(j, hidden + r * D, 4 * (lane + G * j), D);
-            if constexpr (ADD) bn[j] = load_at<SURE>(j, branch + r * D, 4 * (lane + G * j), D);
-        }
-    };
-    const bool drops = ADD && a.branch.kept < 65536u, drops_out = a.out.kept < 65536u;
-    Bits last0 = {0, 0}, last1 = {0, 0};   // of the last of an odd number of chunks, where a draw gave it in advance
-    bool ahead = false;
-    if (row < a.N) fetch(row);
-    for (; row < a.N; row += step) {
-        const unsigned r32 = static_cast<unsigned>(row);
-        f32x4 h[NCH], br[ADD ? NCH : 1];
-#pragma unroll
-        for (int j = 0; j < NCH; ++j) {
-            h[j] = widen_at<SURE>(j, hn[j], 4 * (lane + G * j), D);
-            if constexpr (ADD) br[j] = widen_at<SURE>(j, bn[j], 4 * (lane + G * j), D);
-        }
-        if (row + step < a.N) fetch(row + step);
-        Bits bits = {0, 0};
-        if constexpr (NCH & 1) {
-            if (drops && drops_out) {
-                last_draws<G, NCH>(k0, k1, r32, lane, last0, bits);
-            } else if (drops || drops_out) {
-                if (!ahead) last_draws<G, NCH>(drops ? k0 : k1, r32, static_cast<unsigned>(row + step), lane, bits, last1);
-                else bits = last1;
-                ahead = !ahead;
-                last0 = bits;
-            }
-        }
-        if constexpr (ADD) {
-            if (drops) {
-                pair_draws<G, NCH>(k0, r32, lane, [&](int j, Bits b) { br[j] = drop_group(br[j], b.lo, b.hi, a.branch); });
-                if constexpr (NCH & 1) br[NCH - 1] = drop_group(br[NCH - 1], last0.lo, last0.hi, a.branch);
-            }
-#pragma unroll
-            for (int j = 0; j < NCH; ++j) {
-                h[j] = round_group<TH>(h[j] + br[j]);
-                store_at<SURE>(j, sum + row * D, 4 * (lane + G * j), D, h[j]);
-            }
-        }
-        float mean = 0.f, s = 0.f;
-        if (a.layer) {
-#pragma unroll
-            for (int j = 0; j < NCH; ++j) s = sum4(h[j], s);
-            mean = row_sum<G>(s, slots[0], lane) * inv_d;
-            s = 0.f;
-        }
-#pragma unroll
-        for (int j = 0; j < NCH; ++j) {
-            h[j] = j < SURE ? h[j] - mean : inside<false>(h[j] - mean, 4 * (lane + G * j), D);
-            s = sq4(h[j], s);
-        }
-        const float r = 1.0f / __fsqrt_rn(row_sum<G>(s, slots[1], lane) * inv_d + a.eps);
-        if (a.stats && lane == 0) {
-            a.stats[2 * row] = mean;
-            a.stats[2 * row + 1] = r;
-        }
-#pragma unroll
-        for (int j = 0; j < NCH; ++j) h[j] = fma4(h[j] * r, w[j], b[j]);
-        if (drops_out) {
-            pair_draws<G, NCH>(k1, r32, lane, [&](int j, Bits b) { h[j] = keep_group(h[j], b.lo, b.hi, a.out.kept); });
-            if constexpr (NCH & 1) h[NCH - 1] = keep_group(h[NCH - 1], bits.lo, bits.hi, a.out.kept);
-        }
-#pragma unroll
-        for (int j = 0; j < NCH; ++j) store_at<SURE>(j, out + row * D, 4 * (lane + G * j), D, h[j]);
-        if constexpr (std::is_same<TO, float>::value && 4 * G * NCH <= 2048) {   // what the searches take of fp32 rows
-            if (a.xx || a.img.rows) {
-                float m = 0.f, inv;
-                s = 0.f;
-                if constexpr (G <= 64) {
-                    // 16 lanes: chunk j is what lanes 16 j .. 16 j + 15 of a wave hold, added by its steps of 32 and 16
-                    float q[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int j = 0; j < NCH; ++j) {
-                        q[G < 64 ? j : 0] = sq4(h[j], q[G < 64 ? j : 0]);
-                        m = t5vq_absmax4(m, h[j].x, h[j].y, h[j].z, h[j].w);
-                    }
-                    s = G < 64 ? (q[0] + q[2]) + (q[1] + q[3]) : q[0];
-                } else {   // a row's norm is defined on one wave's lanes: through LDS, every wave adds all of it
-#pragma unroll
-                    for (int j = 0; j < NCH; ++j) copy[lane + G * j] = h[j];
-                    __syncthreads();
-#pragma unroll
-                    for (int q = 0; q < G * NCH; q += 64) {
-                        const f32x4 v = copy[(lane & 63) + q];
-                        s = sq4(v, s);
-                        m = t5vq_absmax4(m, v.x, v.y, v.z, v.w);
-                    }
-                }
-                s = lanes_sum<(G < 64 ? G : 64)>(s);
-                if (a.xx && lane == 0) a.xx[row] = s;
-                if (a.img.rows) {
-#pragma unroll
-                    for (int o = (G < 64 ? G : 64) / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-                    const float sc = t5vq_image_scale(m, &inv);
-                    if (lane == 0) a.img.inv[row] = inv;
-#pragma unroll
-                    for (int j = 0; j < NCH; ++j) {
-                        const unsigned q = lane + G * j;
-                        if (4 * q < D) t5vq_image_store4(a.img.rows + row * D, q, h[j].x, h[j].y, h[j].z, h[j].w, sc);
-                    }
-                }
-            }
-        }
-        if constexpr (G > 64) __syncthreads();   // the next row's sums reuse the slots
-    }
-}
-
-__device__ __forceinline__ float block_sum(float v, float* slots) {   // 256 threads; fixed order
-    v = wave_sum(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) slots[threadIdx.x >> 6] = v;
-    __syncthreads();
-    return (slots[0] + slots[1]) + (slots[2] + slots[3]);
-}
-
-// Rows that registers do not hold (D > 16384), and rows shorter than one group (D < 4): one workgroup per row, read again from memory for each of its sums.
-template <class TH, class TB, class TO, bool ADD>
-__global__ __launch_bounds__(256) void norm_rows_kernel(const TH* __restrict__ hidden, const TB* __restrict__ branch,
-                                                        TO* __restrict__ out, TH* __restrict__ sum, NormArgs a) {
-    __shared__ float slots[4];
-    const int tid = threadIdx.x, D = a.D;
-    if (a.ctr.ticket_out && blockIdx.x == 0 && tid == 0) give_ticket(a.ctr);
-    const bool drops = ADD && a.branch.kept < 65536u;
-    const Key k0 = site_key(a.ctr, 0), k1 = site_key(a.ctr, 1);
-    for (long long row = blockIdx.x; row < a.N; row += gridDim.x) {
-        auto group = [&](int q) {
-            f32x4 h = load_group(hidden + row * D, 4 * q, D);
-            if constexpr (ADD) {
-                f32x4 b = load_group(branch + row * D, 4 * q, D);
-                if (drops) b = drop_at(b, k0, q, static_cast<unsigned>(row), a.branch);
-                h = round_group<TH>(h + b);
-            }
-            return h;
-        };
-        const int groups = (D + 3) / 4;
-        float s = 0.f, mean = 0.f;
-        if (a.layer) {
-            for (int q = tid; q < groups; q += 256) s = sum4(group(q), s);
-            mean = block_sum(s, slots) / static_cast<float>(D);
-        }
-        s = 0.f;
-        for (int q = tid; q < groups; q += 256) {
-            const f32x4 h = group(q);
-            if constexpr (ADD) store_group(sum + row * D, 4 * q, D, h);
-            f32x4 d = h - mean;
-            if (4 * q + 1 >= D) d.y = 0.f;
-            if (4 * q + 2 >= D) d.z = 0.f;
-            if (4 * q + 3 >= D) d.w = 0.f;
-            s = sq4(d, s);
-        }
-        const float r = 1.0f / __fsqrt_rn(block_sum(s, slots) / static_cast<float>(D) + a.eps);
-        if (a.stats && tid == 0) {
-            a.stats[2 * row] = mean;
-            a.stats[2 * row + 1] = r;
-        }
-        for (int q = tid; q < groups; q += 256) {
-            f32x4 y = (group(q) - mean) * r * load_param(a.weight, a.weight_type, 4 * q, D);
-            if (a.bias) y += load_param(a.bias, a.weight_type, 4 * q, D);
-            if (a.out.kept < 65536u) y = drop_at(y, k1, q, static_cast<unsigned>(row), a.out);
-            store_group(out + row * D, 4 * q, D, y);
-        }
-    }
-}
-
-template <class TH, class TB, class TO, bool ADD, int G, int NCH, bool FULL>
-void go(const void* hidden, const void* branch, void* out, void* sum, const NormArgs& a, hipStream_t stream) {
-    constexpr auto kernel = norm_kernel<TH, TB, TO, ADD, G, NCH, FULL>;
-    constexpr int threads = G > 256 ? G : 256;
-    static const int64_t most = CUS * resident(kernel, threads);
-    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(workgroups(a.N, threads / G, most))), dim3(threads), 0, stream,
-                       static_cast<const TH*>(hidden), static_cast<const TB*>(branch), static_cast<TO*>(out),
-                       static_cast<TH*>(sum), a);
-}
-
-template <class TH, class TB, class TO, bool ADD>
-void launch_norm(const void* hidden, const void* branch, void* out, void* sum, const NormArgs& a, hipStream_t stream) {
-#define T5VQ_NK(G, NCH)                                                                                        \
-    (a.D == 4 * G * NCH ? go<TH, TB, TO, ADD, G, NCH, true>(hidden, branch, out, sum, a, stream)               \
-                        : go<TH, TB, TO, ADD, G, NCH, false>(hidden, branch, out, sum, a, stream))
-    if (a.D < 4 || a.D > 16384)
-        hipLaunchKernelGGL((norm_rows_kernel<TH, TB, TO, ADD>), dim3(static_cast<unsigned>(workgroups(a.N, 1, CUS * 8))),
-                           dim3(256), 0, stream, static_cast<const TH*>(hidden), static_cast<const TB*>(branch),
-                           static_cast<TO*>(out), static_cast<TH*>(sum), a);
-    else if (a.D <= 64) T5VQ_NK(16, 1);
-    else if (a.D <= 128) T5VQ_NK(16, 2);
-    else if (a.D <= 192) T5VQ_NK(16, 3);
-    else if (a.D <= 256) T5VQ_NK(16, 4);
-    else if (a.D <= 512) T5VQ_NK(64, 2);
-    else if (a.D <= 768) T5VQ_NK(64, 3);
-    else if (a.D <= 1024) T5VQ_NK(64, 4);
-    else if (a.D <= 2048) T5VQ_NK(256, 2);
-    else if (a.D <= 4096) T5VQ_NK(256, 4);
-    else if (a.D <= 8192) T5VQ_NK(1024, 2);
-    else T5VQ_NK(1024, 4);
-#undef T5VQ_NK
+    if (s0 || col >= D) return;
+    acc = sums[0][c];
+    if (type == T5VQ_F32) static_cast<float*>(to)[col] = acc;
+    else if (type == T5VQ_BF16) static_cast<__bf16*>(to)[col] = static_cast<__bf16>(acc);
+    else static_cast<_Float16*>(to)[col] = static_cast<_Float16>(acc);
 }
 
 template <class TX, class TY>
@@ -408,19 +193,61 @@ int t5vq_norm_forward(const void* hidden, int hidden_type, const void* branch, i
              reinterpret_cast<long long*>(ticket_out)};
     a.stats = stats, a.xx = xx, a.img = t5vq_token_image_parts(token_image, N, D);
     hipStream_t s = static_cast<hipStream_t>(stream);
-#define T5VQ_NF(H, B, O, ADD) launch_norm<H, B, O, ADD>(hidden, branch, out, sum, a, s)
-#define T5VQ_NF_HALF(H)                                                                         \
-    (out_type == T5VQ_F32 ? (branch ? T5VQ_NF(H, H, float, true) : T5VQ_NF(H, H, float, false)) \
-                          : (branch ? T5VQ_NF(H, H, H, true) : T5VQ_NF(H, H, H, false)))
-    if (hidden_type == T5VQ_BF16) T5VQ_NF_HALF(__bf16);
-    else if (hidden_type == T5VQ_F16) T5VQ_NF_HALF(_Float16);
-    else if (!branch) T5VQ_NF(float, float, float, false);
-    else if (branch_type == T5VQ_F32) T5VQ_NF(float, float, float, true);
-    else if (branch_type == T5VQ_BF16) T5VQ_NF(float, __bf16, float, true);
-    else T5VQ_NF(float, _Float16, float, true);
-#undef T5VQ_NF_HALF
-#undef T5VQ_NF
+    (hidden_type == T5VQ_F32    ? forward_f32
+     : hidden_type == T5VQ_BF16 ? forward_bf16
+                                : forward_f16)(hidden, branch, branch_type, out, out_type, sum, a, s);
     T5VQ_I_CHECK_HIP(hipGetLastError());
+    return T5VQ_OK;
+}
+
+int64_t t5vq_norm_backward_workspace_bytes(int64_t N, int64_t D) {
+    return N > 0 && D > 0 ? slices_of(N) * 2 * D * 4 : 0;
+}
+
+int t5vq_norm_backward(const void* grad_out, int out_type, const void* grad_sum, const void* h, int hidden_type,
+                       const void* weight, int weight_type, int norm_kind, const float* stats, int64_t N, int64_t D,
+                       double branch_p, double p, const int64_t* ticket, void* grad_hidden, void* grad_branch,
+                       int branch_type, void* grad_weight, void* grad_bias, void* workspace, int64_t workspace_bytes,
+                       t5vq_stream_t stream) {
+    T5VQ_I_REQUIRE(grad_out && h && weight && stats && grad_hidden, "null pointer");
+    T5VQ_I_REQUIRE(known_type(hidden_type) && known_type(weight_type) && known_type(out_type), "unknown element type");
+    T5VQ_I_REQUIRE(out_type == hidden_type || out_type == T5VQ_F32, "grad_out is of hidden's type or fp32");
+    T5VQ_I_REQUIRE(!grad_branch || branch_type == hidden_type || (hidden_type == T5VQ_F32 && known_type(branch_type)),
+                   "branch is of hidden's type, or hidden is fp32");
+    T5VQ_I_REQUIRE(norm_kind == T5VQ_NORM_LAYER || norm_kind == T5VQ_NORM_RMS, "unknown norm");
+    T5VQ_I_REQUIRE(N > 0 && N <= (1LL << 32) - 1 && D > 0 && D <= (1LL << 30), "N, D out of range");
+    const int64_t kept0 = t5vq_dropout_keep_count(branch_p), kept1 = t5vq_dropout_keep_count(p);
+    T5VQ_I_REQUIRE(kept0 >= 0 && kept1 >= 0, "p must be in [0, 1]");
+    T5VQ_I_REQUIRE(ticket || (kept1 == 65536 && (!grad_branch || kept0 == 65536)), "dropout needs the forward's ticket");
+    T5VQ_I_REQUIRE(aligned_to(grad_out, out_type) && aligned_to(h, hidden_type) && aligned_to(weight, weight_type) &&
+                       aligned_to(grad_hidden, hidden_type) && (!grad_sum || aligned_to(grad_sum, hidden_type)) &&
+                       (!grad_branch || aligned_to(grad_branch, branch_type)) &&
+                       (!grad_weight || aligned_to(grad_weight, weight_type)) &&
+                       (!grad_bias || aligned_to(grad_bias, weight_type)),
+                   "elements must be aligned");
+    const bool params = grad_weight || grad_bias;
+    T5VQ_I_REQUIRE(!params || (workspace && workspace_bytes >= t5vq_norm_backward_workspace_bytes(N, D) &&
+                               aligned_to(workspace, T5VQ_F32)),
+                   "parameter gradients need a workspace of t5vq_norm_backward_workspace_bytes(N, D)");
+    BackArgs a;
+    a.weight = weight, a.weight_type = weight_type, a.layer = norm_kind == T5VQ_NORM_LAYER;
+    a.D = static_cast<int>(D), a.N = N;
+    a.branch = make_drop(branch_p), a.out = make_drop(p);
+    a.ctr = {0, 0, reinterpret_cast<const long long*>(ticket), ticket ? reinterpret_cast<const long long*>(ticket) + 1 : nullptr,
+             nullptr};
+    a.stats = stats, a.grad_weight = grad_weight, a.grad_bias = grad_bias;
+    float* part = params ? static_cast<float*>(workspace) : nullptr;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const int64_t slices = (hidden_type == T5VQ_F32    ? backward_f32
+                            : hidden_type == T5VQ_BF16 ? backward_bf16
+                                                       : backward_f16)(grad_out, out_type, grad_sum, h, a, grad_hidden,
+                                                                       grad_branch, branch_type, part, s);
+    T5VQ_I_CHECK_HIP(hipGetLastError());
+    if (params && slices) {
+        hipLaunchKernelGGL(norm_param_reduce_kernel, dim3(static_cast<unsigned>((D + 15) / 16), 2), dim3(1024), 0, s, part,
+                           static_cast<int>(slices), a.D, grad_weight, grad_bias, weight_type);
+        T5VQ_I_CHECK_HIP(hipGetLastError());
+    }
     return T5VQ_OK;
 }
 

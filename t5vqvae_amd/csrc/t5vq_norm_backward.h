@@ -1,45 +1,25 @@
-// t5vq_norm_backward.hip -- gradients of the norms of t5vq_norm.hip.  gfx950 kernels + C ABI; include/t5vq.h has the contract.
-//
-// Compiled with -ffp-contract=off: every fused multiply-add below is an explicit fmaf().
+// Internal to libt5vq.so: the backward kernels of the norms (t5vq_norm_f32 / _bf16 / _f16.hip instantiate them).
+#ifndef T5VQ_NORM_BACKWARD_H_
+#define T5VQ_NORM_BACKWARD_H_
 #include "t5vq_norm.h"
 
-using namespace t5vq_norm;
-
-namespace {
-
-struct BackArgs {
-    const void* weight;
-    int weight_type, layer, D;
-    long long N;
-    Drop branch, out;
-    Counter ctr;
-    const float* stats;   // [N, 2]
-    void *grad_weight, *grad_bias;
-};
-
-__device__ __forceinline__ float block_sum(float v, float* slots) {   // 256 threads; fixed order
-    v = wave_sum(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) slots[threadIdx.x >> 6] = v;
-    __syncthreads();
-    return (slots[0] + slots[1]) + (slots[2] + slots[3]);
-}
+namespace t5vq_norm {
 
 // With gy = kept ? g * scale : 0, a = gy * weight, n = (h - mean) r:
 //   grad_h = r (a - mean(a) - n mean(a n)) (+ g_sum), without mean(a) for rms;  grad_branch = kept ? grad_h * scale : 0;
 //   grad_weight = sum over rows of gy n, grad_bias = sum of gy.
 // The row stays in registers between its two sums and its gradients (group lane + G * j in chunk j, as forward), and a wave
 // adds up the parameters' gradients of all rows it walks: every input is read once.  Workgroup b leaves its sums in part[b].
-template <class TO, class TH, class TB, int G, int NCH, int WG, bool FULL>
+template <class TO, class TH, class TB, bool ADD, int G, int NCH, int WG, int MODE>
 __global__ __launch_bounds__(WG) void norm_backward_kernel(const TO* __restrict__ g, const TH* __restrict__ g_sum,
                                                                      const TH* __restrict__ h, BackArgs a,
                                                                      TH* __restrict__ grad_h, TB* __restrict__ grad_branch,
                                                                      float* __restrict__ part) {
-    constexpr int ROWS = WG / G, SURE = sure<G, NCH, FULL>();
+    constexpr int ROWS = WG / G, SURE = sure<G, NCH, MODE>();
     __shared__ float slots[2][G > 64 ? ROWS : 1][G > 64 ? G / 64 : 1];
     __shared__ f32x4 sums[ROWS > 1 ? ROWS : 1][ROWS > 1 ? G * NCH : 1];
     const Place<G, WG> at;
-    const unsigned lane = at.lane, D = FULL ? 4 * G * NCH : a.D;
+    const unsigned lane = at.lane, D = MODE != RAGGED ? 4 * G * NCH : a.D;
     const Key k0 = site_key(a.ctr, 0), k1 = site_key(a.ctr, 1);
     const f32x4 zero4 = {0.f, 0.f, 0.f, 0.f};
     f32x4 w[NCH], gw[NCH], gb[NCH];   // w times the output's scale; gw, gb without it until the end
@@ -53,22 +33,22 @@ __global__ __launch_bounds__(WG) void norm_backward_kernel(const TO* __restrict_
     const long long step = static_cast<long long>(gridDim.x) * ROWS;
     const long long first = static_cast<long long>(blockIdx.x) * ROWS;
     typename Group<TO>::type vn[NCH];
-    typename Group<TH>::type nn[NCH], sn[NCH];
+    typename Group<TH>::type nn[NCH], sn[ADD ? NCH : 1];
     float mean_n = 0.f, r_n = 0.f;
     auto fetch = [&](long long t) {
 #pragma unroll
         for (int j = 0; j < NCH; ++j) {
-            vn[j] = load_at<SURE>(j, g + t * D, 4 * (lane + G * j), D);
-            nn[j] = load_at<SURE>(j, h + t * D, 4 * (lane + G * j), D);
+            vn[j] = load_at<SURE, MODE == STREAMED>(j, g + t * D, 4 * (lane + G * j), D);
+            nn[j] = load_at<SURE, MODE == STREAMED>(j, h + t * D, 4 * (lane + G * j), D);
         }
-        if (g_sum) {
+        if (ADD && g_sum) {
 #pragma unroll
-            for (int j = 0; j < NCH; ++j) sn[j] = load_at<SURE>(j, g_sum + t * D, 4 * (lane + G * j), D);
+            for (int j = 0; j < (ADD ? NCH : 0); ++j) sn[j] = load_at<SURE, MODE == STREAMED>(j, g_sum + t * D, 4 * (lane + G * j), D);
         }
         mean_n = a.stats[2 * t];
         r_n = a.stats[2 * t + 1];
     };
-    const bool drops = grad_branch && a.branch.kept < 65536u, drops_out = a.out.kept < 65536u;
+    const bool drops = ADD && grad_branch && a.branch.kept < 65536u, drops_out = a.out.kept < 65536u;
     Bits last0 = {0, 0}, last1 = {0, 0};   // of the last of an odd number of chunks, where a draw gave it in advance
     bool ahead = false;
     if (first + at.sub < a.N) fetch(first + at.sub);
@@ -78,12 +58,12 @@ __global__ __launch_bounds__(WG) void norm_backward_kernel(const TO* __restrict_
         const bool live = row < a.N;
         if (G <= 64 && !live) break;
         f32x4 v[NCH], n[NCH];
-        typename Group<TH>::type gs[NCH];
+        typename Group<TH>::type gs[ADD ? NCH : 1];
 #pragma unroll
         for (int j = 0; j < NCH; ++j) {
             v[j] = live ? widen_at<SURE>(j, vn[j], 4 * (lane + G * j), D) : zero4;
             n[j] = live ? widen_at<SURE>(j, nn[j], 4 * (lane + G * j), D) : zero4;
-            gs[j] = sn[j];
+            if constexpr (ADD) gs[j] = sn[j];
         }
         const float mean = mean_n, r = r_n;
         if (row + step < a.N) fetch(row + step);
@@ -121,16 +101,17 @@ __global__ __launch_bounds__(WG) void norm_backward_kernel(const TO* __restrict_
 #pragma unroll
         for (int j = 0; j < NCH; ++j) {
             v[j] = fma4(n[j], zero4 - s2, v[j] - s1) * r;
-            if (g_sum) v[j] += widen_at<SURE>(j, gs[j], 4 * (lane + G * j), D);
-            if (live) store_at<SURE>(j, grad_h + row * D, 4 * (lane + G * j), D, v[j]);
+            if constexpr (ADD)
+                if (g_sum) v[j] += widen_at<SURE>(j, gs[j], 4 * (lane + G * j), D);
+            if (live) store_at<SURE, MODE == STREAMED>(j, grad_h + row * D, 4 * (lane + G * j), D, v[j]);
         }
-        if (grad_branch && live) {
+        if (ADD && grad_branch && live) {
             if (drops) {
                 pair_draws<G, NCH>(k0, r32, lane, [&](int j, Bits b) { v[j] = drop_group(v[j], b.lo, b.hi, a.branch); });
                 if constexpr (NCH & 1) v[NCH - 1] = drop_group(v[NCH - 1], last0.lo, last0.hi, a.branch);
             }
 #pragma unroll
-            for (int j = 0; j < NCH; ++j) store_at<SURE>(j, grad_branch + row * D, 4 * (lane + G * j), D, v[j]);
+            for (int j = 0; j < NCH; ++j) store_at<SURE, MODE == STREAMED>(j, grad_branch + row * D, 4 * (lane + G * j), D, v[j]);
         }
         if constexpr (G > 64) __syncthreads();   // the next row's sums reuse the slots
     }
@@ -226,38 +207,10 @@ __global__ __launch_bounds__(256) void norm_param_grad_kernel(const TO* __restri
     store_group(p + D, 4 * q, D, gb);
 }
 
-// part[slices][2][D] to the two gradients: 16 columns x 64 slice groups a workgroup, one tree over the groups -- a fixed order
-__global__ __launch_bounds__(1024) void norm_param_reduce_kernel(const float* __restrict__ part, int slices, int D,
-                                                                 void* __restrict__ grad_weight,
-                                                                 void* __restrict__ grad_bias, int type) {
-    __shared__ float sums[64][17];
-    const int c = threadIdx.x & 15, s0 = threadIdx.x >> 4, col = blockIdx.x * 16 + c;
-    void* to = blockIdx.y ? grad_bias : grad_weight;
-    if (!to) return;
-    const float* p = part + static_cast<size_t>(blockIdx.y) * D + col;
-    float acc = 0.f;
-    if (col < D)
-        for (int s = s0; s < slices; s += 64) acc += p[static_cast<size_t>(s) * 2 * D];
-    sums[s0][c] = acc;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        __syncthreads();
-        if (s0 < o) sums[s0][c] += sums[s0 + o][c];
-    }
-    if (s0 || col >= D) return;
-    acc = sums[0][c];
-    if (type == T5VQ_F32) static_cast<float*>(to)[col] = acc;
-    else if (type == T5VQ_BF16) static_cast<__bf16*>(to)[col] = static_cast<__bf16>(acc);
-    else static_cast<_Float16*>(to)[col] = static_cast<_Float16>(acc);
-}
-
-// How many workgroups share the rows at most; each leaves 2 D floats of sums.
-int64_t slices_of(int64_t N) { return N < 2 * CUS ? N : 2 * CUS; }
-
-template <class TO, class TH, class TB, int G, int NCH, int WG, bool FULL>
+template <class TO, class TH, class TB, bool ADD, int G, int NCH, int WG, int MODE>
 int64_t go(const void* g, const void* g_sum, const void* h, const BackArgs& a, void* grad_h, void* grad_branch, float* part,
            hipStream_t s) {
-    constexpr auto kernel = norm_backward_kernel<TO, TH, TB, G, NCH, WG, FULL>;
+    constexpr auto kernel = norm_backward_kernel<TO, TH, TB, ADD, G, NCH, WG, MODE>;
     static const int64_t most = CUS * resident(kernel, WG);
     // up to four rows a wave one workgroup takes them all: its turns cost less than a second launch
     const int64_t wgs = a.N <= 4 * (WG / G) && part ? 1 : workgroups(a.N, WG / G, most < 2 * CUS ? most : 2 * CUS);
@@ -267,26 +220,32 @@ int64_t go(const void* g, const void* g_sum, const void* h, const BackArgs& a, v
     return wgs > 1 ? wgs : 0;
 }
 
-// Returns how many slices of parameter sums there are in part to be added (0: the gradients are written already).
-template <class TO, class TH, class TB>
+// ADD: with a gradient of the sum or for the branch.
+template <class TO, class TH, class TB, bool ADD>
 int64_t launch_back(const void* g, const void* g_sum, const void* h, const BackArgs& a, void* grad_h, void* grad_branch,
                     float* part, hipStream_t s) {
-// WG, WG2: one workgroup fills a CU with the waves that its registers leave room for (occupancy 2 .. 4 of a SIMD's 512
-// registers), so that few workgroups leave sums behind; whole rows of the half types need the fewest registers.
-#define T5VQ_NBK(G, NCH, WG, WG2)                                                                                  \
-    (a.D == 4 * G * NCH ? go<TO, TH, TB, G, NCH, sizeof(TH) == 2 ? WG2 : WG, true>(g, g_sum, h, a, grad_h, grad_branch, part, s) \
-                        : go<TO, TH, TB, G, NCH, WG, false>(g, g_sum, h, a, grad_h, grad_branch, part, s))
+    const int64_t bytes = a.N * a.D * static_cast<int64_t>(sizeof(TO) + 2 * sizeof(TH) + (g_sum ? sizeof(TH) : 0) +
+                                                           (grad_branch ? sizeof(TB) : 0));
+// One workgroup fills a CU with the waves that its registers leave room for (occupancy 2 .. 4 of a SIMD's 512 registers), so
+// that few workgroups leave sums behind: WG threads, W for whole rows of a half type, P for whole fp32 rows of a plain norm.
+#define T5VQ_NBK(G, NCH, WG, W, P)                                                                                           \
+    do {                                                                                                                     \
+        constexpr int T = sizeof(TH) == 2 ? W : ADD ? WG : P;                                                                \
+        return a.D != 4 * G * NCH      ? go<TO, TH, TB, ADD, G, NCH, WG, RAGGED>(g, g_sum, h, a, grad_h, grad_branch, part, s) \
+               : bytes < STREAM_BYTES ? go<TO, TH, TB, ADD, G, NCH, T, WHOLE>(g, g_sum, h, a, grad_h, grad_branch, part, s)  \
+                                      : go<TO, TH, TB, ADD, G, NCH, T, STREAMED>(g, g_sum, h, a, grad_h, grad_branch, part, s); \
+    } while (0)
     if (a.D >= 4 && a.D <= 8192) {
-        if (a.D <= 64) return T5VQ_NBK(16, 1, 768, 768);
-        if (a.D <= 128) return T5VQ_NBK(16, 2, 768, 768);
-        if (a.D <= 192) return T5VQ_NBK(16, 3, 768, 768);
-        if (a.D <= 256) return T5VQ_NBK(16, 4, 512, 512);
-        if (a.D <= 512) return T5VQ_NBK(64, 2, 768, 768);
-        if (a.D <= 768) return T5VQ_NBK(64, 3, 768, 1024);
-        if (a.D <= 1024) return T5VQ_NBK(64, 4, 512, 768);
-        if (a.D <= 2048) return T5VQ_NBK(256, 2, 1024, 1024);
-        if (a.D <= 4096) return T5VQ_NBK(256, 4, 512, 768);
-        return T5VQ_NBK(1024, 2, 1024, 1024);
+        if (a.D <= 64) T5VQ_NBK(16, 1, 768, 768, 768);
+        if (a.D <= 128) T5VQ_NBK(16, 2, 768, 768, 768);
+        if (a.D <= 192) T5VQ_NBK(16, 3, 768, 768, 768);
+        if (a.D <= 256) T5VQ_NBK(16, 4, 512, 512, 512);
+        if (a.D <= 512) T5VQ_NBK(64, 2, 768, 768, 768);
+        if (a.D <= 768) T5VQ_NBK(64, 3, 768, 1024, 1024);
+        if (a.D <= 1024) T5VQ_NBK(64, 4, 512, 768, 768);
+        if (a.D <= 2048) T5VQ_NBK(256, 2, 1024, 1024, 1024);
+        if (a.D <= 4096) T5VQ_NBK(256, 4, 512, 768, 512);
+        return go<TO, TH, TB, ADD, 1024, 2, 1024, RAGGED>(g, g_sum, h, a, grad_h, grad_branch, part, s);
     }
 #undef T5VQ_NBK
     hipLaunchKernelGGL((norm_backward_rows_kernel<TO, TH, TB>), dim3(static_cast<unsigned>(workgroups(a.N, 1, CUS * 8))),
@@ -299,64 +258,5 @@ int64_t launch_back(const void* g, const void* g_sum, const void* h, const BackA
     return slices;
 }
 
-}  // namespace
-
-extern "C" {
-
-int64_t t5vq_norm_backward_workspace_bytes(int64_t N, int64_t D) {
-    return N > 0 && D > 0 ? slices_of(N) * 2 * D * 4 : 0;
-}
-
-int t5vq_norm_backward(const void* grad_out, int out_type, const void* grad_sum, const void* h, int hidden_type,
-                       const void* weight, int weight_type, int norm_kind, const float* stats, int64_t N, int64_t D,
-                       double branch_p, double p, const int64_t* ticket, void* grad_hidden, void* grad_branch,
-                       int branch_type, void* grad_weight, void* grad_bias, void* workspace, int64_t workspace_bytes,
-                       t5vq_stream_t stream) {
-    T5VQ_I_REQUIRE(grad_out && h && weight && stats && grad_hidden, "null pointer");
-    T5VQ_I_REQUIRE(known_type(hidden_type) && known_type(weight_type) && known_type(out_type), "unknown element type");
-    T5VQ_I_REQUIRE(out_type == hidden_type || out_type == T5VQ_F32, "grad_out is of hidden's type or fp32");
-    T5VQ_I_REQUIRE(!grad_branch || branch_type == hidden_type || (hidden_type == T5VQ_F32 && known_type(branch_type)),
-                   "branch is of hidden's type, or hidden is fp32");
-    T5VQ_I_REQUIRE(norm_kind == T5VQ_NORM_LAYER || norm_kind == T5VQ_NORM_RMS, "unknown norm");
-    T5VQ_I_REQUIRE(N > 0 && N <= (1LL << 32) - 1 && D > 0 && D <= (1LL << 30), "N, D out of range");
-    const int64_t kept0 = t5vq_dropout_keep_count(branch_p), kept1 = t5vq_dropout_keep_count(p);
-    T5VQ_I_REQUIRE(kept0 >= 0 && kept1 >= 0, "p must be in [0, 1]");
-    T5VQ_I_REQUIRE(ticket || (kept1 == 65536 && (!grad_branch || kept0 == 65536)), "dropout needs the forward's ticket");
-    T5VQ_I_REQUIRE(aligned_to(grad_out, out_type) && aligned_to(h, hidden_type) && aligned_to(weight, weight_type) &&
-                       aligned_to(grad_hidden, hidden_type) && (!grad_sum || aligned_to(grad_sum, hidden_type)) &&
-                       (!grad_branch || aligned_to(grad_branch, branch_type)) &&
-                       (!grad_weight || aligned_to(grad_weight, weight_type)) &&
-                       (!grad_bias || aligned_to(grad_bias, weight_type)),
-                   "elements must be aligned");
-    const bool params = grad_weight || grad_bias;
-    T5VQ_I_REQUIRE(!params || (workspace && workspace_bytes >= t5vq_norm_backward_workspace_bytes(N, D) &&
-                               aligned_to(workspace, T5VQ_F32)),
-                   "parameter gradients need a workspace of t5vq_norm_backward_workspace_bytes(N, D)");
-    BackArgs a;
-    a.weight = weight, a.weight_type = weight_type, a.layer = norm_kind == T5VQ_NORM_LAYER;
-    a.D = static_cast<int>(D), a.N = N;
-    a.branch = make_drop(branch_p), a.out = make_drop(p);
-    a.ctr = {0, 0, reinterpret_cast<const long long*>(ticket), ticket ? reinterpret_cast<const long long*>(ticket) + 1 : nullptr,
-             nullptr};
-    a.stats = stats, a.grad_weight = grad_weight, a.grad_bias = grad_bias;
-    float* part = params ? static_cast<float*>(workspace) : nullptr;
-    int64_t slices = 0;
-    hipStream_t s = static_cast<hipStream_t>(stream);
-#define T5VQ_NB(O, H, B) slices = launch_back<O, H, B>(grad_out, grad_sum, h, a, grad_hidden, grad_branch, part, s)
-    if (hidden_type == T5VQ_BF16) out_type == T5VQ_F32 ? T5VQ_NB(float, __bf16, __bf16) : T5VQ_NB(__bf16, __bf16, __bf16);
-    else if (hidden_type == T5VQ_F16)
-        out_type == T5VQ_F32 ? T5VQ_NB(float, _Float16, _Float16) : T5VQ_NB(_Float16, _Float16, _Float16);
-    else if (!grad_branch || branch_type == T5VQ_F32) T5VQ_NB(float, float, float);
-    else if (branch_type == T5VQ_BF16) T5VQ_NB(float, float, __bf16);
-    else T5VQ_NB(float, float, _Float16);
-#undef T5VQ_NB
-    T5VQ_I_CHECK_HIP(hipGetLastError());
-    if (params && slices) {
-        hipLaunchKernelGGL(norm_param_reduce_kernel, dim3(static_cast<unsigned>((D + 15) / 16), 2), dim3(1024), 0, s, part,
-                           static_cast<int>(slices), a.D, grad_weight, grad_bias, weight_type);
-        T5VQ_I_CHECK_HIP(hipGetLastError());
-    }
-    return T5VQ_OK;
-}
-
-}  // extern "C"
+}  // namespace t5vq_norm
+#endif

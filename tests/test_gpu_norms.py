@@ -181,7 +181,7 @@ def test_dropout_behind_four_gigabytes():
 
 # ---- norms, forward ---------------------------------------------------------------------------------------------------
 SHAPES = [(1, 1), (1, 768), (5, 3), (37, 64), (30, 130), (45, 771), (64, 1024), (9, 2048), (7, 2051), (3, 4096), (2, 8200),
-          (1, 20001), (2880, 768), (33, 190), (50, 256), (10, 300)]
+          (1, 20001), (2880, 768), (33, 190), (50, 256), (10, 300), (21, 513)]
 
 
 @pytest.mark.parametrize("n,d", SHAPES)
@@ -339,7 +339,8 @@ def test_gradients_are_the_slopes_of_the_forward(kind):
 
 
 # ---- outputs for the searches --------------------------------------------------------------------------------------------
-@pytest.mark.parametrize("n,d", [(1, 64), (45, 768), (130, 2048), (33, 100), (257, 1024), (64, 1536), (31, 192), (50, 256), (7, 140)])
+@pytest.mark.parametrize("n,d", [(1, 64), (45, 768), (130, 2048), (33, 100), (257, 1024), (64, 1536), (31, 192), (50, 256), (7, 140),
+                                 (9, 300), (12, 512), (5, 640)])
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_row_norms_and_image_are_those_of_the_searches(n, d, dtype):
     from t5vqvae_amd import ops
