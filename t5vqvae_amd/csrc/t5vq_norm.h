@@ -20,6 +20,14 @@ template <> struct Group<float> { typedef float type __attribute__((ext_vector_t
 template <> struct Group<__bf16> { typedef __bf16 type __attribute__((ext_vector_type(4), aligned(2))); };
 template <> struct Group<_Float16> { typedef _Float16 type __attribute__((ext_vector_type(4), aligned(2))); };
 
+// What a row kernel knows of its rows: that they fill their chunks exactly (WHOLE), and then that a call moves so much that
+// the caches keep nothing of it (STREAMED: reads and writes go past them).
+enum { RAGGED, WHOLE, STREAMED };
+// Measured with every call's output kept (us; in brackets the call and a kernel that reads its output): 65536 x 768 bf16 norm,
+// 201 MB, 42.2 -> 39.8 (75.9 -> 71.4), its backward, 302 MB, 65.5 -> 59.6 (101 -> 91); 65536 x 768 fp32 norm 80 -> 74;
+// 16384 x 768 fp32 norm, 101 MB, 23.4 -> 21.0 (37.2 -> 39.0): below, the neighbour loses what it would find in the cache.
+constexpr int64_t STREAM_BYTES = 192ll << 20;
+
 // eight elements: a Philox block's columns
 template <class T> struct Octet;
 template <> struct Octet<float> { typedef float type __attribute__((ext_vector_type(8), aligned(4))); };
@@ -58,14 +66,23 @@ __device__ __forceinline__ void store_group(T* __restrict__ row, unsigned c, uns
         if (c + 2 < D) row[c + 2] = static_cast<T>(v.z);
     }
 }
-// chunk j of a row whose chunks below SURE are whole (j known when unrolled); STREAM: past the caches
-template <int SURE, bool STREAM = false, class T>
+template <int MODE, class V>
+__device__ __forceinline__ V read(const V* p) {
+    if constexpr (MODE == STREAMED) return __builtin_nontemporal_load(p);
+    else return *p;
+}
+template <int MODE, class V>
+__device__ __forceinline__ void write(V* p, V v) {
+    if constexpr (MODE == STREAMED) __builtin_nontemporal_store(v, p);
+    else *p = v;
+}
+// chunk j of a row whose chunks below SURE are whole (j known when unrolled)
+template <int SURE, int MODE = WHOLE, class T>
 __device__ __forceinline__ void store_at(int j, T* __restrict__ row, unsigned c, unsigned D, f32x4 v) {
     typedef typename Group<T>::type V;
     if (j < SURE || c + 4 <= D) {   // the row's pointer is the wave's, the lane's place 32 bits: one scalar base, one offset
         V* p = reinterpret_cast<V*>(reinterpret_cast<char*>(row) + c * static_cast<unsigned>(sizeof(T)));
-        if constexpr (STREAM) __builtin_nontemporal_store(__builtin_convertvector(v, V), p);
-        else *p = __builtin_convertvector(v, V);
+        write<MODE>(p, __builtin_convertvector(v, V));
     } else {
         store_group<false>(row, c, D, v);
     }
@@ -73,12 +90,10 @@ __device__ __forceinline__ void store_at(int j, T* __restrict__ row, unsigned c,
 // Reads of the other chunks do not branch (a branch would wait for every read already on its way): a group that reaches past
 // the row's end, or lies behind it, reads the row's last four elements (D >= 4), and widen_at puts them in their places
 // when they are there, 0 behind the end.
-template <int SURE, bool STREAM = false, class T>
+template <int SURE, int MODE = WHOLE, class T>
 __device__ __forceinline__ typename Group<T>::type load_at(int j, const T* __restrict__ row, unsigned c, unsigned D) {
     const unsigned at = (j < SURE || c + 4 <= D ? c : D - 4) * static_cast<unsigned>(sizeof(T));
-    const auto* p = reinterpret_cast<const typename Group<T>::type*>(reinterpret_cast<const char*>(row) + at);
-    if constexpr (STREAM) return __builtin_nontemporal_load(p);
-    else return *p;
+    return read<MODE>(reinterpret_cast<const typename Group<T>::type*>(reinterpret_cast<const char*>(row) + at));
 }
 template <int SURE, class V>
 __device__ __forceinline__ f32x4 widen_at(int j, V raw, unsigned c, unsigned D) {
@@ -274,14 +289,6 @@ __device__ __forceinline__ void last_draws(Key k, unsigned row, unsigned next, u
     const bool odd = lane & 1;
     share(philox(k, (lane >> 1) + (G / 2) * (NCH - 1), odd ? next : row), odd, now, then);
 }
-
-// What a row kernel knows of its rows: that they fill their chunks exactly (WHOLE), and then that a call moves so much that
-// the caches keep nothing of it (STREAMED: reads and writes go past them).
-enum { RAGGED, WHOLE, STREAMED };
-// From 1.5 times the 256 MB of the last cache: 65536 x 768 fp32 rms norm 77 -> 73 us, its backward 124 -> 117 us, add + norm
-// 155 -> 145 us and backward 206 -> 194 us; below, what a neighbouring kernel left there is lost (16384 x 768 fp32 norm
-// 17 -> 21 us, 65536 x 768 bf16 backward, 300 MB, 61 -> 66 us).
-constexpr int64_t STREAM_BYTES = 384ll << 20;
 
 // Where a thread stands: G lanes a row, WG threads a workgroup.  With a row to every wave or more the row is the wave's, and
 // kept in scalar registers.

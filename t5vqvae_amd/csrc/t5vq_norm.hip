@@ -10,12 +10,13 @@ namespace {
 
 // y = residual + (kept ? x * scale : 0).  A thread takes U blocks of eight columns, 256 blocks apart, so that each Philox block
 // is drawn once and U blocks of every input are on their way together.  WHOLE: D % 8 == 0, rows follow each other without
-// a gap and a block is one access of 16 (half types) or two (fp32).
-template <class TX, class TY, bool RES, bool WHOLE>
+// a gap and a block of a half type is one access of 16 bytes.
+template <class TX, class TY, bool RES, int MODE>
 __global__ __launch_bounds__(256) void dropout_add_kernel(const TX* __restrict__ x, const TY* __restrict__ res, unsigned D,
                                                           unsigned blocks, Quotient per_row, Drop drop, Counter ctr,
                                                           TY* __restrict__ y) {
     constexpr int U = 2;
+    constexpr bool WHOLE = MODE != RAGGED;
     if (ctr.ticket_out && blockIdx.x == 0 && threadIdx.x == 0) give_ticket(ctr);
     const unsigned first = blockIdx.x * (256u * U) + threadIdx.x;
     typename Octet<TX>::type xv[U];
@@ -30,8 +31,8 @@ __global__ __launch_bounds__(256) void dropout_add_kernel(const TX* __restrict__
         blk[u] = b - row[u] * per_row.d;
         at[u] = WHOLE ? static_cast<size_t>(b) * 8 : static_cast<size_t>(row[u]) * D;
         if constexpr (WHOLE) {
-            xv[u] = *reinterpret_cast<const typename Octet<TX>::type*>(x + at[u]);
-            if constexpr (RES) rv[u] = *reinterpret_cast<const typename Octet<TY>::type*>(res + at[u]);
+            xv[u] = read<MODE>(reinterpret_cast<const typename Octet<TX>::type*>(x + at[u]));
+            if constexpr (RES) rv[u] = read<MODE>(reinterpret_cast<const typename Octet<TY>::type*>(res + at[u]));
         } else {
             xv[u] = load_octet(x + at[u], blk[u] * 8, D);     // D >= 4, see load_at
             if constexpr (RES) rv[u] = load_octet(res + at[u], blk[u] * 8, D);
@@ -55,13 +56,51 @@ __global__ __launch_bounds__(256) void dropout_add_kernel(const TX* __restrict__
         }
         if constexpr (WHOLE) {
             typedef typename Octet<TY>::type V;
-            *reinterpret_cast<V*>(y + at[u]) =
-                __builtin_convertvector(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), V);
+            write<MODE>(reinterpret_cast<V*>(y + at[u]),
+                        __builtin_convertvector(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), V));
         } else {
             store_group(y + at[u], c, D, lo);
             store_group(y + at[u], c + 4, D, hi);
         }
     }
+}
+
+// The same for whole blocks with fp32 on either side, where a block is two accesses: a wave takes 64 blocks as two times 64
+// groups, so that each of its accesses is 1 KB without a gap, and neighbouring lanes share their draws.
+template <class TX, class TY, bool RES, int MODE>
+__global__ __launch_bounds__(256) void dropout_add_wide_kernel(const TX* __restrict__ x, const TY* __restrict__ res,
+                                                               unsigned blocks, Quotient per_row, Drop drop, Counter ctr,
+                                                               TY* __restrict__ y) {
+    if (ctr.ticket_out && blockIdx.x == 0 && threadIdx.x == 0) give_ticket(ctr);
+    const unsigned lane = threadIdx.x & 63, base = blockIdx.x * 256u + (threadIdx.x & ~63u);   // the wave's first block
+    const bool odd = lane & 1;
+    f32x4 v[2];
+    typename Group<TY>::type rv[2];
+    bool there[2];
+    size_t at[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        there[i] = base + 32 * i + (lane >> 1) < blocks;
+        at[i] = (static_cast<size_t>(base) * 2 + 64 * i + lane) * 4;
+        if (there[i]) {
+            v[i] = widen(read<MODE>(reinterpret_cast<const typename Group<TX>::type*>(x + at[i])));
+            if constexpr (RES) rv[i] = read<MODE>(reinterpret_cast<const typename Group<TY>::type*>(res + at[i]));
+        }
+    }
+    if (drop.kept < 65536u) {
+        const unsigned b = base + (odd ? 32 : 0) + (lane >> 1), row = per_row.of(b);
+        Bits bits[2];
+        share(philox(site_key(ctr, 0), b - row * per_row.d, row), odd, bits[0], bits[1]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) v[i] = drop_group(v[i], bits[i].lo, bits[i].hi, drop);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        if (there[i]) {
+            typedef typename Group<TY>::type V;
+            if constexpr (RES) v[i] = widen(rv[i]) + v[i];
+            write<MODE>(reinterpret_cast<V*>(y + at[i]), __builtin_convertvector(v[i], V));
+        }
 }
 
 // rows of one to three columns: a thread each
@@ -102,27 +141,37 @@ __global__ __launch_bounds__(1024) void norm_param_reduce_kernel(const float* __
     else static_cast<_Float16*>(to)[col] = static_cast<_Float16>(acc);
 }
 
-template <class TX, class TY>
-void launch_dropout(const void* x, const void* res, void* y, int64_t N, int64_t D, Drop drop, const Counter& ctr,
+template <class TX, class TY, bool RES>
+void launch_dropout(const void* x_, const void* res_, void* y_, int64_t N, int64_t D, Drop drop, const Counter& ctr,
                     hipStream_t stream) {
-    const int64_t per_row = (D + 7) / 8, blocks = N * per_row;
-#define T5VQ_DK(RES, WHOLE)                                                                                          \
-    hipLaunchKernelGGL((dropout_add_kernel<TX, TY, RES, WHOLE>), dim3(static_cast<unsigned>((blocks + 511) / 512)), \
-                       dim3(256), 0, stream, static_cast<const TX*>(x), static_cast<const TY*>(res),                \
-                       static_cast<unsigned>(D), static_cast<unsigned>(blocks),                                      \
-                       quotient_by(static_cast<unsigned>(per_row)), drop, ctr, static_cast<TY*>(y))
+    const TX* x = static_cast<const TX*>(x_);
+    const TY* res = static_cast<const TY*>(res_);
+    TY* y = static_cast<TY*>(y_);
+    const int64_t per_row = (D + 7) / 8, bytes = N * D * static_cast<int64_t>(sizeof(TX) + (RES ? 2 : 1) * sizeof(TY));
+    const unsigned blocks = static_cast<unsigned>(N * per_row), d = static_cast<unsigned>(D);
+    const Quotient q = quotient_by(static_cast<unsigned>(per_row));
+    const dim3 two((blocks + 511u) / 512u), one((blocks + 255u) / 256u);
     if (D < 4) {
         hipLaunchKernelGGL((dropout_add_short_kernel<TX, TY>), dim3(static_cast<unsigned>((N + 255) / 256)), dim3(256), 0, stream,
-                           static_cast<const TX*>(x), static_cast<const TY*>(res), static_cast<unsigned>(D), N, drop, ctr,
-                           static_cast<TY*>(y));
-    } else if (D % 8 == 0) {
-        if (res) T5VQ_DK(true, true);
-        else T5VQ_DK(false, true);
+                           x, res, d, N, drop, ctr, y);
+    } else if (D % 8) {
+        hipLaunchKernelGGL((dropout_add_kernel<TX, TY, RES, RAGGED>), two, dim3(256), 0, stream, x, res, d, blocks, q, drop, ctr,
+                           y);
+    } else if constexpr (sizeof(TX) == 4 || sizeof(TY) == 4) {
+        if (bytes < STREAM_BYTES)
+            hipLaunchKernelGGL((dropout_add_wide_kernel<TX, TY, RES, WHOLE>), one, dim3(256), 0, stream, x, res, blocks, q, drop,
+                               ctr, y);
+        else
+            hipLaunchKernelGGL((dropout_add_wide_kernel<TX, TY, RES, STREAMED>), one, dim3(256), 0, stream, x, res, blocks, q,
+                               drop, ctr, y);
     } else {
-        if (res) T5VQ_DK(true, false);
-        else T5VQ_DK(false, false);
+        if (bytes < STREAM_BYTES)
+            hipLaunchKernelGGL((dropout_add_kernel<TX, TY, RES, WHOLE>), two, dim3(256), 0, stream, x, res, d, blocks, q, drop,
+                               ctr, y);
+        else
+            hipLaunchKernelGGL((dropout_add_kernel<TX, TY, RES, STREAMED>), two, dim3(256), 0, stream, x, res, d, blocks, q, drop,
+                               ctr, y);
     }
-#undef T5VQ_DK
 }
 
 }  // namespace
@@ -150,7 +199,9 @@ int t5vq_dropout_add(const void* x, int x_type, const void* residual, int64_t N,
                          reinterpret_cast<const long long*>(seed_dev), reinterpret_cast<const long long*>(offset_dev),
                          reinterpret_cast<long long*>(ticket_out)};
     hipStream_t s = static_cast<hipStream_t>(stream);
-#define T5VQ_DA(X, Y) launch_dropout<X, Y>(x, residual, y, N, D, drop, ctr, s)
+#define T5VQ_DA(X, Y) \
+    (residual ? launch_dropout<X, Y, true>(x, residual, y, N, D, drop, ctr, s) \
+              : launch_dropout<X, Y, false>(x, residual, y, N, D, drop, ctr, s))
     if (x_type == T5VQ_F32 && y_type == T5VQ_F32) T5VQ_DA(float, float);
     else if (x_type == T5VQ_BF16 && y_type == T5VQ_BF16) T5VQ_DA(__bf16, __bf16);
     else if (x_type == T5VQ_F16 && y_type == T5VQ_F16) T5VQ_DA(_Float16, _Float16);

@@ -38,12 +38,12 @@ __global__ __launch_bounds__(WG) void norm_backward_kernel(const TO* __restrict_
     auto fetch = [&](long long t) {
 #pragma unroll
         for (int j = 0; j < NCH; ++j) {
-            vn[j] = load_at<SURE, MODE == STREAMED>(j, g + t * D, 4 * (lane + G * j), D);
-            nn[j] = load_at<SURE, MODE == STREAMED>(j, h + t * D, 4 * (lane + G * j), D);
+            vn[j] = load_at<SURE, MODE>(j, g + t * D, 4 * (lane + G * j), D);
+            nn[j] = load_at<SURE, MODE>(j, h + t * D, 4 * (lane + G * j), D);
         }
         if (ADD && g_sum) {
 #pragma unroll
-            for (int j = 0; j < (ADD ? NCH : 0); ++j) sn[j] = load_at<SURE, MODE == STREAMED>(j, g_sum + t * D, 4 * (lane + G * j), D);
+            for (int j = 0; j < (ADD ? NCH : 0); ++j) sn[j] = load_at<SURE, MODE>(j, g_sum + t * D, 4 * (lane + G * j), D);
         }
         mean_n = a.stats[2 * t];
         r_n = a.stats[2 * t + 1];
@@ -103,7 +103,7 @@ __global__ __launch_bounds__(WG) void norm_backward_kernel(const TO* __restrict_
             v[j] = fma4(n[j], zero4 - s2, v[j] - s1) * r;
             if constexpr (ADD)
                 if (g_sum) v[j] += widen_at<SURE>(j, gs[j], 4 * (lane + G * j), D);
-            if (live) store_at<SURE, MODE == STREAMED>(j, grad_h + row * D, 4 * (lane + G * j), D, v[j]);
+            if (live) store_at<SURE, MODE>(j, grad_h + row * D, 4 * (lane + G * j), D, v[j]);
         }
         if (ADD && grad_branch && live) {
             if (drops) {
@@ -111,7 +111,7 @@ __global__ __launch_bounds__(WG) void norm_backward_kernel(const TO* __restrict_
                 if constexpr (NCH & 1) v[NCH - 1] = drop_group(v[NCH - 1], last0.lo, last0.hi, a.branch);
             }
 #pragma unroll
-            for (int j = 0; j < NCH; ++j) store_at<SURE, MODE == STREAMED>(j, grad_branch + row * D, 4 * (lane + G * j), D, v[j]);
+            for (int j = 0; j < NCH; ++j) store_at<SURE, MODE>(j, grad_branch + row * D, 4 * (lane + G * j), D, v[j]);
         }
         if constexpr (G > 64) __syncthreads();   // the next row's sums reuse the slots
     }

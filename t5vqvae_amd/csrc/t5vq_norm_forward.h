@@ -35,8 +35,8 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void norm_kernel(const TH* __res
     auto fetch = [&](long long r) {
 #pragma unroll
         for (int j = 0; j < NCH; ++j) {
-            hn[j] = load_at<SURE, MODE == STREAMED>(j, hidden + r * D, 4 * (lane + G * j), D);
-            if constexpr (ADD) bn[j] = load_at<SURE, MODE == STREAMED>(j, branch + r * D, 4 * (lane + G * j), D);
+            hn[j] = load_at<SURE, MODE>(j, hidden + r * D, 4 * (lane + G * j), D);
+            if constexpr (ADD) bn[j] = load_at<SURE, MODE>(j, branch + r * D, 4 * (lane + G * j), D);
         }
     };
     const bool drops = ADD && a.branch.kept < 65536u, drops_out = a.out.kept < 65536u;
@@ -71,7 +71,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void norm_kernel(const TH* __res
 #pragma unroll
             for (int j = 0; j < NCH; ++j) {
                 h[j] = round_group<TH>(h[j] + br[j]);
-                store_at<SURE, MODE == STREAMED>(j, sum + row * D, 4 * (lane + G * j), D, h[j]);
+                store_at<SURE, MODE>(j, sum + row * D, 4 * (lane + G * j), D, h[j]);
             }
         }
         float mean = 0.f, s = 0.f;
@@ -98,7 +98,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void norm_kernel(const TH* __res
             if constexpr (NCH & 1) h[NCH - 1] = keep_group(h[NCH - 1], bits.lo, bits.hi, a.out.kept);
         }
 #pragma unroll
-        for (int j = 0; j < NCH; ++j) store_at<SURE, MODE == STREAMED>(j, out + row * D, 4 * (lane + G * j), D, h[j]);
+        for (int j = 0; j < NCH; ++j) store_at<SURE, MODE>(j, out + row * D, 4 * (lane + G * j), D, h[j]);
         if constexpr (std::is_same<TO, float>::value && 4 * G * NCH <= 2048) {   // what the searches take of fp32 rows
             if (a.xx || a.img.rows) {
                 float m = 0.f, inv;
