@@ -18,6 +18,8 @@ __global__ __launch_bounds__(WG) void norm_backward_kernel(const TO* __restrict_
     constexpr int ROWS = WG / G, SURE = sure<G, NCH, MODE>();
     __shared__ float slots[2][G > 64 ? ROWS : 1][G > 64 ? G / 64 : 1];
     __shared__ f32x4 sums[ROWS > 1 ? ROWS : 1][ROWS > 1 ? G * NCH : 1];
+    // a workgroup's waves keep step where they share a row, and past the caches, where rows that are read together lie together
+    constexpr bool TOGETHER = G > 64 || MODE == STREAMED;
     const Place<G, WG> at;
     const unsigned lane = at.lane, D = MODE != RAGGED ? 4 * G * NCH : a.D;
     const Key k0 = site_key(a.ctr, 0), k1 = site_key(a.ctr, 1);
@@ -56,7 +58,7 @@ __global__ __launch_bounds__(WG) void norm_backward_kernel(const TO* __restrict_
         const long long row = base + at.sub;
         // where waves wait for each other every one of them comes along, with a row of its own or without
         const bool live = row < a.N;
-        if (G <= 64 && !live) break;
+        if (!TOGETHER && !live) break;
         f32x4 v[NCH], n[NCH];
         typename Group<TH>::type gs[ADD ? NCH : 1];
 #pragma unroll
@@ -113,7 +115,7 @@ __global__ __launch_bounds__(WG) void norm_backward_kernel(const TO* __restrict_
 #pragma unroll
             for (int j = 0; j < NCH; ++j) store_at<SURE, MODE>(j, grad_branch + row * D, 4 * (lane + G * j), D, v[j]);
         }
-        if constexpr (G > 64) __syncthreads();   // the next row's sums reuse the slots
+        if constexpr (TOGETHER) __syncthreads();   // the next row's sums reuse the slots
     }
     if (!part) return;
     float* p = part + static_cast<size_t>(blockIdx.x) * 2 * D;

@@ -195,7 +195,9 @@ template <class TH, class TB, class TO, bool ADD, int G, int NCH, int MODE>
 void go(const void* hidden, const void* branch, void* out, void* sum, const NormArgs& a, hipStream_t stream) {
     constexpr auto kernel = norm_kernel<TH, TB, TO, ADD, G, NCH, MODE>;
     constexpr int threads = G > 256 ? G : 256;
-    static const int64_t most = CUS * resident(kernel, threads);
+    // past the caches four times as many as the card holds: handed out in order, they keep closer together in memory than
+    // workgroups that walk the rows alone (65536 x 768 fp32 norm 73.8 -> 69.2 us, add + norm 147 -> 141 us)
+    static const int64_t most = CUS * resident(kernel, threads) * (MODE == STREAMED ? 4 : 1);
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(workgroups(a.N, threads / G, most))), dim3(threads), 0, stream,
                        static_cast<const TH*>(hidden), static_cast<const TB*>(branch), static_cast<TO*>(out),
                        static_cast<TH*>(sum), a);

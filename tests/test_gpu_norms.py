@@ -338,6 +338,47 @@ def test_gradients_are_the_slopes_of_the_forward(kind):
         assert abs(got - slope) <= 1e-5 * size, (i, got, slope)
 
 
+@pytest.mark.parametrize("n,d,dtype", [(65541, 768, F32), (131083, 768, BF16), (800005, 64, F32), (50003, 1024, F16),
+                                       (25003, 2048, F32)])
+def test_large_calls_equal_their_parts(n, d, dtype):
+    """Calls that go past the caches (192 MB and more) against the same rows in small calls, bit for bit, and the oracle's
+    masks on the last rows; the parameters' gradients against float64 sums."""
+    from t5vqvae_amd import ops
+    g = torch.Generator(device="cuda").manual_seed(n)
+    h, br, go, gs = (torch.randn(n, d, generator=g, device="cuda").to(dtype) for _ in range(4))
+    w, b = torch.randn(d, generator=g, device="cuda"), torch.randn(d, generator=g, device="cuda")
+    last = [(0, 37), (n // 2, 61), (n - 29, 29)]
+    out, total, stats, _, _ = ops.norm_forward(h, w, b, kind="layer", eps=EPS, branch=br)
+    got = ops.norm_backward(go, gs, total, w, stats, kind="layer", branch_dtype=dtype)
+    res = ops.dropout_add(br, 0.0, h)[0]
+    assert torch.equal(res, total)
+    for first, count in last:
+        part = slice(first, first + count)
+        o, t, s, _, _ = ops.norm_forward(h[part], w, b, kind="layer", eps=EPS, branch=br[part])
+        assert torch.equal(o, out[part]) and torch.equal(t, total[part]) and torch.equal(s, stats[part])
+        x = ops.norm_backward(go[part], gs[part], t, w, s, kind="layer", branch_dtype=dtype)
+        assert torch.equal(x[0], got[0][part]) and torch.equal(x[1], got[1][part])
+    unit = (total.double() - stats[:, :1].double()) * stats[:, 1:].double()
+    # n is off by 2 u |n| (a subtraction and a product); a column's chain: a wave's rows (n / 2048 at least three), 16 waves,
+    # the tree over up to 512 slices
+    chain_rows = n / 2048 + 64
+    for grad, terms in ((got[2], go.double() * unit), (got[3], go.double())):
+        want, size = terms.sum(0), terms.abs().sum(0)
+        assert bool(((grad.double() - want).abs() <= (chain_rows + 4) * U * size).all())
+    del unit, terms, res, total, got, out
+    p = 0.25
+    y = ops.dropout_add(torch.ones_like(h), p, None, ticket())[0]
+    o, t, s, _, _ = ops.norm_forward(h, w, b, kind="rms", eps=EPS, branch=br, branch_p=p, p=p, ticket=ticket())
+    gh, gb, _, _ = ops.norm_backward(go, gs, t, w, s, kind="rms", branch_p=p, p=p, ticket=ticket(), branch_dtype=dtype)
+    for first, count in last:
+        keep0 = no.keep_mask(count, d, p, TICKET, 0, first_row=first)
+        keep1 = no.keep_mask(count, d, p, TICKET, 1, first_row=first)
+        part = slice(first, first + count)
+        assert torch.equal(y[part].cpu() != 0, keep0)
+        check_forward(o[part], t[part], w, b, "rms", keep1, p, dtype)
+        check_backward((gh[part], gb[part], None, None), go[part], t[part], w, "rms", keep1, p, gs[part], keep0, p)
+
+
 # ---- outputs for the searches --------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("n,d", [(1, 64), (45, 768), (130, 2048), (33, 100), (257, 1024), (64, 1536), (31, 192), (50, 256), (7, 140),
                                  (9, 300), (12, 512), (5, 640)])
