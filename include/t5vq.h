@@ -426,7 +426,9 @@ int t5vq_rmsnorm_sqnorms_img_f32(const float* hidden, const float* gamma, const 
  *   *offset_dev is ADDED to offset -- a generator that a graph replays, or an earlier call's ticket.  ticket_out
  *   (nullable) receives the {seed, offset} the call drew with; backward calls take it as `ticket`.  Site 0 is a dropout
  *   by itself or that of the branch, site 1 that of a norm's output; a call uses offset .. offset + 7, so calls whose
- *   offsets are 8 apart share no numbers. */
+ *   offsets are 8 apart share no numbers.
+ * Ranges: N < 2^32, D <= 2^30 (dropout: N * ceil(D / 8) <= 2^32 - 512).  Outputs overlap no input and no other output; all
+ * tensors are dense, their elements aligned to the element's size. */
 #define T5VQ_F32 0
 #define T5VQ_BF16 1
 #define T5VQ_F16 2

@@ -174,6 +174,11 @@ void launch_dropout(const void* x_, const void* res_, void* y_, int64_t N, int64
     }
 }
 
+// whether a call may write its ticket while others of its workgroups still read where it draws from
+bool apart(const int64_t* out, const int64_t* seed, const int64_t* offset) {
+    return !out || (seed != out && seed != out + 1 && offset != out && offset != out + 1);
+}
+
 }  // namespace
 
 extern "C" {
@@ -194,6 +199,8 @@ int t5vq_dropout_add(const void* x, int x_type, const void* residual, int64_t N,
     T5VQ_I_REQUIRE(t5vq_dropout_keep_count(p) >= 0, "p must be in [0, 1]");
     T5VQ_I_REQUIRE(aligned_to(x, x_type) && aligned_to(y, y_type) && (!residual || aligned_to(residual, y_type)),
                    "elements must be aligned");
+    T5VQ_I_REQUIRE(y != x && y != residual, "y must not be an input");
+    T5VQ_I_REQUIRE(apart(ticket_out, seed_dev, offset_dev), "ticket_out must not be what the call draws from");
     const Drop drop = make_drop(p);
     const Counter ctr = {static_cast<unsigned long long>(seed), static_cast<unsigned long long>(offset),
                          reinterpret_cast<const long long*>(seed_dev), reinterpret_cast<const long long*>(offset_dev),
@@ -232,6 +239,9 @@ int t5vq_norm_forward(const void* hidden, int hidden_type, const void* branch, i
                        (!bias || aligned_to(bias, weight_type)) &&
                        (!branch || (aligned_to(branch, branch_type) && aligned_to(sum, hidden_type))),
                    "elements must be aligned");
+    T5VQ_I_REQUIRE(out != hidden && out != branch && (!branch || (sum != hidden && sum != branch && sum != out)),
+                   "outputs must not be inputs, or each other");
+    T5VQ_I_REQUIRE(apart(ticket_out, seed_dev, offset_dev), "ticket_out must not be what the call draws from");
     T5VQ_I_REQUIRE((!xx && !token_image) || (out_type == T5VQ_F32 && D % 4 == 0 && D <= 2048),
                    "row norms and images are those of fp32 rows, D % 4 == 0, D <= 2048");
     T5VQ_I_REQUIRE((reinterpret_cast<uintptr_t>(token_image) & 255u) == 0, "token_image must be 256-byte aligned");
@@ -276,6 +286,9 @@ int t5vq_norm_backward(const void* grad_out, int out_type, const void* grad_sum,
                        (!grad_weight || aligned_to(grad_weight, weight_type)) &&
                        (!grad_bias || aligned_to(grad_bias, weight_type)),
                    "elements must be aligned");
+    T5VQ_I_REQUIRE(grad_hidden != grad_out && grad_hidden != grad_sum && grad_hidden != h && grad_hidden != grad_branch &&
+                       (!grad_branch || (grad_branch != grad_out && grad_branch != grad_sum && grad_branch != h)),
+                   "outputs must not be inputs, or each other");
     const bool params = grad_weight || grad_bias;
     T5VQ_I_REQUIRE(!params || (workspace && workspace_bytes >= t5vq_norm_backward_workspace_bytes(N, D) &&
                                aligned_to(workspace, T5VQ_F32)),

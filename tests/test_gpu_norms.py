@@ -584,6 +584,25 @@ def test_captured_steps_draw_anew_and_match_their_tickets():
                                                                 br.cpu() * np.float32(no.scale_of(p)), torch.zeros(()))))
 
 
+def test_first_call_of_a_kernel_inside_a_capture():
+    """No warm-up: a kernel's first call (which asks how many workgroups the card holds) may be a captured one."""
+    from t5vqvae_amd import ops
+    h, g, w = rows(40, 5000, 201, F16).cuda(), rows(40, 5000, 202, F16).cuda(), rows(1, 5000, 203, F16)[0].cuda()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, _, stats, _, _ = ops.norm_forward(h, w, kind="rms", eps=EPS)
+        back = ops.norm_backward(g, None, h, w, stats, kind="rms", want_bias=False)
+        drop = ops.dropout_add(h, 0.5, None, None)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        check_forward(out, h, w, None, "rms", None, 0.0, F16)
+        check_backward(back, g, h, w, "rms", None, 0.0)
+        keep = no.keep_mask(40, 5000, 0.5, drop[1].tolist(), 0)
+        assert torch.equal(drop[0].cpu(), torch.where(keep, h.cpu() * 2, torch.zeros((), dtype=F16)))
+
+
 def test_two_graphs_of_the_same_operators_replay_beside_each_other():
     """Two graphs captured from the same call, replayed in turn on two streams: no shared workspace."""
     from t5vqvae_amd import ops

@@ -58,33 +58,35 @@ def test_c_abi_refuses_bad_calls_before_any_launch():
     lib = _lib.load()
     buf = ctypes.create_string_buffer(4096)
     p = ctypes.c_void_p((ctypes.addressof(buf) + 255) // 256 * 256)
-    odd = ctypes.c_void_p(p.value + 1)
+    odd, y_, z_ = (ctypes.c_void_p(p.value + k) for k in (1, 512, 1024))
     F32, BF16, F16, LAYER, RMS = 0, 1, 2, 0, 1
 
-    def drop(x=p, xt=F32, res=None, n=4, d=8, prob=0.1, y=p, yt=F32):
-        return lib.t5vq_dropout_add(x, xt, res, n, d, prob, 1, 0, None, None, None, y, yt, None)
+    def drop(x=p, xt=F32, res=None, n=4, d=8, prob=0.1, y=y_, yt=F32, sd=None, od=None, to=None):
+        return lib.t5vq_dropout_add(x, xt, res, n, d, prob, 1, 0, sd, od, to, y, yt, None)
 
     for call in (dict(x=None), dict(y=None), dict(xt=3), dict(yt=-1), dict(xt=BF16, yt=F16), dict(n=0), dict(n=1 << 32),
                  dict(d=0), dict(d=(1 << 30) + 1), dict(n=(1 << 32) - 1, d=16), dict(prob=-0.1), dict(prob=1.5),
-                 dict(prob=math.nan), dict(x=odd), dict(y=odd), dict(res=odd)):
+                 dict(prob=math.nan), dict(x=odd), dict(y=odd), dict(res=odd),
+                 dict(y=p), dict(res=y_), dict(sd=z_, to=z_), dict(od=z_, to=z_)):
         assert drop(**call) == 1, call
         assert lib.t5vq_last_error()
 
-    def fwd(h=p, ht=F32, b=None, bt=F32, w=p, bias=None, wt=F32, kind=LAYER, eps=1e-6, n=4, d=8, bp=0.0, prob=0.0, out=p,
-            ot=F32, total=None, xx=None, img=None):
-        return lib.t5vq_norm_forward(h, ht, b, bt, w, bias, wt, kind, eps, n, d, bp, prob, 1, 0, None, None, None, out, ot,
+    def fwd(h=p, ht=F32, b=None, bt=F32, w=p, bias=None, wt=F32, kind=LAYER, eps=1e-6, n=4, d=8, bp=0.0, prob=0.0, out=y_,
+            ot=F32, total=None, xx=None, img=None, sd=None, to=None):
+        return lib.t5vq_norm_forward(h, ht, b, bt, w, bias, wt, kind, eps, n, d, bp, prob, 1, 0, sd, None, to, out, ot,
                                      total, None, xx, img, None)
 
     for call in (dict(h=None), dict(w=None), dict(out=None), dict(b=p), dict(ht=7), dict(wt=7), dict(ot=7),
-                 dict(ht=F32, ot=BF16), dict(ht=BF16, ot=F16), dict(ht=BF16, ot=BF16, b=p, bt=F32, total=p),
-                 dict(b=p, bt=5, total=p), dict(kind=2), dict(eps=-1e-6), dict(eps=math.nan), dict(n=0), dict(n=1 << 32),
+                 dict(ht=F32, ot=BF16), dict(ht=BF16, ot=F16), dict(ht=BF16, ot=BF16, b=p, bt=F32, total=z_),
+                 dict(b=p, bt=5, total=z_), dict(kind=2), dict(eps=-1e-6), dict(eps=math.nan), dict(n=0), dict(n=1 << 32),
                  dict(d=0), dict(bp=1.5), dict(prob=-0.5), dict(prob=math.nan), dict(h=odd), dict(w=odd), dict(out=odd),
-                 dict(bias=odd), dict(b=odd, total=p), dict(b=p, total=odd), dict(xx=p, d=6), dict(xx=p, d=4096),
+                 dict(bias=odd), dict(b=odd, total=z_), dict(b=p, total=odd), dict(out=p), dict(b=p, total=p), dict(b=p, total=y_),
+                 dict(b=y_, total=z_), dict(sd=z_, to=z_), dict(xx=p, d=6), dict(xx=p, d=4096),
                  dict(xx=p, ht=BF16, ot=BF16), dict(img=odd)):
         assert fwd(**call) == 1, call
         assert lib.t5vq_last_error()
 
-    def back(g=p, ot=F32, gs=None, h=p, ht=F32, w=p, wt=F32, kind=LAYER, st=p, n=4, d=8, bp=0.0, prob=0.0, ticket=None, gh=p,
+    def back(g=p, ot=F32, gs=None, h=p, ht=F32, w=p, wt=F32, kind=LAYER, st=p, n=4, d=8, bp=0.0, prob=0.0, ticket=None, gh=y_,
              gb=None, bt=F32, gw=None, gbias=None, ws=None, wsb=0):
         return lib.t5vq_norm_backward(g, ot, gs, h, ht, w, wt, kind, st, n, d, bp, prob, ticket, gh, gb, bt, gw, gbias, ws,
                                       wsb, None)
@@ -92,8 +94,8 @@ def test_c_abi_refuses_bad_calls_before_any_launch():
     need = lib.t5vq_norm_backward_workspace_bytes(4, 8)
     assert need > 0 and lib.t5vq_norm_backward_workspace_bytes(0, 8) == 0
     for call in (dict(g=None), dict(h=None), dict(w=None), dict(st=None), dict(gh=None), dict(ot=BF16), dict(ht=9),
-                 dict(ht=BF16, ot=BF16, gb=p, bt=F32), dict(kind=-1), dict(n=0), dict(d=0), dict(prob=0.1),
-                 dict(gb=p, bp=0.1), dict(prob=2.0, ticket=p), dict(gw=p), dict(gbias=p, ws=p, wsb=need - 1),
+                 dict(ht=BF16, ot=BF16, gb=z_, bt=F32), dict(kind=-1), dict(n=0), dict(d=0), dict(prob=0.1),
+                 dict(gb=z_, bp=0.1), dict(gh=p), dict(gb=p), dict(gb=y_), dict(gs=y_), dict(prob=2.0, ticket=p), dict(gw=p), dict(gbias=p, ws=p, wsb=need - 1),
                  dict(gw=p, ws=odd, wsb=need), dict(g=odd), dict(h=odd), dict(gs=odd), dict(gh=odd), dict(gb=odd),
                  dict(gw=odd, ws=p, wsb=need)):
         assert back(**call) == 1, call
