@@ -102,9 +102,9 @@ __global__ __launch_bounds__(WG) void norm_backward_kernel(const TO* __restrict_
         s2 = row_sum<G>(s2, slots[1][G > 64 ? at.sub : 0], lane) * inv_d;
 #pragma unroll
         for (int j = 0; j < NCH; ++j) {
-            v[j] = fma4(n[j], zero4 - s2, v[j] - s1) * r;
-            if constexpr (ADD)
-                if (g_sum) v[j] += widen_at<SURE>(j, gs[j], 4 * (lane + G * j), D);
+            v[j] = fma4(n[j], zero4 - s2, v[j] - s1);
+            if (ADD && g_sum) v[j] = fma4(v[j], zero4 + r, widen_at<SURE>(j, gs[ADD ? j : 0], 4 * (lane + G * j), D));
+            else v[j] *= r;
             if (live) store_at<SURE, MODE>(j, grad_h + row * D, 4 * (lane + G * j), D, v[j]);
         }
         if (ADD && grad_branch && live) {
