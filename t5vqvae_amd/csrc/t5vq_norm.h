@@ -3,8 +3,7 @@
 //
 // Rows are walked in GROUPS of four consecutive columns: group q = columns 4q .. 4q + 3, one group per lane.  A row of any
 // length starts at any multiple of its element's size, so group accesses promise the compiler no more than the element's
-// alignment (gfx950 reads and writes global memory at any byte address; one 16- or 8-byte access per group all the same);
-// only the last group of a row with D % 4 != 0 goes element by element.
+// alignment (gfx950 reads and writes global memory at any byte address; one 16- or 8-byte access per group all the same).
 #ifndef T5VQ_NORM_H_
 #define T5VQ_NORM_H_
 #include "t5vq_internal.h"
@@ -12,8 +11,6 @@
 namespace t5vq_norm {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
-typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 
 template <class T> struct Group;   // four elements of T in memory, aligned like one
 template <> struct Group<float> { typedef float type __attribute__((ext_vector_type(4), aligned(4))); };
@@ -34,32 +31,26 @@ template <> struct Octet<float> { typedef float type __attribute__((ext_vector_t
 template <> struct Octet<__bf16> { typedef __bf16 type __attribute__((ext_vector_type(8), aligned(2))); };
 template <> struct Octet<_Float16> { typedef _Float16 type __attribute__((ext_vector_type(8), aligned(2))); };
 
-// Columns c .. c + 3 of a row of D elements, as they are in memory; columns >= D read as 0.  FULL: there are none (a row that
-// fills every lane's groups: no comparison, no branch).
-template <bool FULL, class T>
-__device__ __forceinline__ typename Group<T>::type load_raw(const T* __restrict__ row, unsigned c, unsigned D) {
-    typedef typename Group<T>::type V;
-    if (FULL || c + 4 <= D) return *reinterpret_cast<const V*>(row + c);
-    V v = {T(0), T(0), T(0), T(0)};
+template <class V>
+__device__ __forceinline__ f32x4 widen(V v) { return __builtin_convertvector(v, f32x4); }
+// Columns c .. c + 3 of a row of D elements; columns >= D read as 0.  (Branches: for reads that nothing else waits behind.)
+template <class T>
+__device__ __forceinline__ f32x4 load_group(const T* __restrict__ row, unsigned c, unsigned D) {
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (c + 4 <= D) return widen(*reinterpret_cast<const typename Group<T>::type*>(row + c));
     if (c < D) {
-        v.x = row[c];
-        if (c + 1 < D) v.y = row[c + 1];
-        if (c + 2 < D) v.z = row[c + 2];
+        v.x = static_cast<float>(row[c]);
+        if (c + 1 < D) v.y = static_cast<float>(row[c + 1]);
+        if (c + 2 < D) v.z = static_cast<float>(row[c + 2]);
     }
     return v;
 }
-template <class V>
-__device__ __forceinline__ f32x4 widen(V v) { return __builtin_convertvector(v, f32x4); }
-template <bool FULL = false, class T>
-__device__ __forceinline__ f32x4 load_group(const T* __restrict__ row, unsigned c, unsigned D) {
-    return widen(load_raw<FULL>(row, c, D));
-}
-// each value rounded once, to nearest even
-template <bool FULL = false, class T>
+// each value rounded once, to nearest even; columns >= D are not written
+template <class T>
 __device__ __forceinline__ void store_group(T* __restrict__ row, unsigned c, unsigned D, f32x4 v) {
-    if (FULL || c + 4 <= D) {
-        typedef typename Group<T>::type V;
-        *reinterpret_cast<V*>(row + c) = __builtin_convertvector(v, V);
+    if (c + 4 <= D) {
+        typedef typename Group<T>::type G;
+        *reinterpret_cast<G*>(row + c) = __builtin_convertvector(v, G);
     } else if (c < D) {
         row[c] = static_cast<T>(v.x);
         if (c + 1 < D) row[c + 1] = static_cast<T>(v.y);
@@ -84,7 +75,7 @@ __device__ __forceinline__ void store_at(int j, T* __restrict__ row, unsigned c,
         V* p = reinterpret_cast<V*>(reinterpret_cast<char*>(row) + c * static_cast<unsigned>(sizeof(T)));
         write<MODE>(p, __builtin_convertvector(v, V));
     } else {
-        store_group<false>(row, c, D, v);
+        store_group(row, c, D, v);
     }
 }
 // Reads of the other chunks do not branch (a branch would wait for every read already on its way): a group that reaches past
@@ -119,6 +110,7 @@ __device__ __forceinline__ f32x4 round_group(f32x4 v) {   // what a later read o
     typedef T V __attribute__((ext_vector_type(4)));
     return __builtin_convertvector(__builtin_convertvector(v, V), f32x4);
 }
+
 // floor(n / d) of any 32-bit n by a multiplication (Granlund, Montgomery: "Division by invariant integers using
 // multiplication", PLDI 1994, figure 4.1): with l = ceil(log2 d), m = floor(2^32 (2^l - d) / d) + 1 and t = high(m n) the
 // quotient is (t + ((n - t) >> min(l, 1))) >> max(l - 1, 0).
@@ -136,7 +128,7 @@ inline Quotient quotient_by(unsigned d) {
     return {d, m, l ? 1u : 0u, l ? static_cast<unsigned>(l - 1) : 0u};
 }
 
-// a parameter vector whose type is only known at run time (its reads are few: once per row at most, from cache)
+// a parameter vector whose type is only known at run time (read once a workgroup, or from cache)
 __device__ __forceinline__ f32x4 load_param(const void* p, int type, unsigned c, unsigned D) {
     if (type == T5VQ_F32) return load_group(static_cast<const float*>(p), c, D);
     if (type == T5VQ_BF16) return load_group(static_cast<const __bf16*>(p), c, D);
@@ -188,7 +180,9 @@ __device__ __forceinline__ void give_ticket(const Counter& c) {   // by one thre
 struct Words { unsigned w0, w1, w2, w3; };
 // Philox4x32-10 (Salmon, Moraes, Dror, Shaw: "Parallel random numbers: as easy as 1, 2, 3", SC 2011) of the counter
 // (site offset, block of eight columns, row): words 0, 1 belong to the block's lower group of four, 2, 3 to its upper one,
-// 16 bits an element, low half first.  Any lane can draw any element's bits at any time: the mask is never stored.
+// 16 bits an element, low half first.  Any lane can draw any element's bits at any time: the mask is never stored.  A draw is
+// 20 products of 32 x 32 -> 64 bits (v_mad_u64_u32; 15 where the offset and the row are the wave's) and 20 three-way xors,
+// about 110 instructions with its exchange for the 8 elements of two lanes' groups.
 __device__ __forceinline__ Words philox(const Key k, unsigned block, unsigned row) {
     unsigned a = k.c0, b = k.c1, c = block, d = row, k0 = k.k0, k1 = k.k1;
 #pragma unroll
@@ -329,9 +323,8 @@ __device__ __forceinline__ float block_sum(float v, float* slots) {   // 256 thr
     return (slots[0] + slots[1]) + (slots[2] + slots[3]);
 }
 // values of columns >= D to 0 (they only exist in a row's last group and behind it)
-template <bool FULL>
 __device__ __forceinline__ f32x4 inside(f32x4 v, unsigned c, unsigned D) {
-    if (!FULL && c + 4 > D) {
+    if (c + 4 > D) {
         if (c >= D) v.x = 0.f;
         if (c + 1 >= D) v.y = 0.f;
         if (c + 2 >= D) v.z = 0.f;

@@ -10,7 +10,8 @@ namespace {
 
 // y = residual + (kept ? x * scale : 0).  A thread takes U blocks of eight columns, 256 blocks apart, so that each Philox block
 // is drawn once and U blocks of every input are on their way together.  WHOLE: D % 8 == 0, rows follow each other without
-// a gap and a block of a half type is one access of 16 bytes.
+// a gap and a block of a half type is one access of 16 bytes.  HBM-bound: 65536 x 768 bf16 with a residual 48 us = 6.3 TB/s, of
+// which the draws' issue fills 21; rows of 513 fp16 16.9 -> 18.9 us with them.
 template <class TX, class TY, bool RES, int MODE>
 __global__ __launch_bounds__(256) void dropout_add_kernel(const TX* __restrict__ x, const TY* __restrict__ res, unsigned D,
                                                           unsigned blocks, Quotient per_row, Drop drop, Counter ctr,
@@ -66,7 +67,8 @@ __global__ __launch_bounds__(256) void dropout_add_kernel(const TX* __restrict__
 }
 
 // The same for whole blocks with fp32 on either side, where a block is two accesses: a wave takes 64 blocks as two times 64
-// groups, so that each of its accesses is 1 KB without a gap, and neighbouring lanes share their draws.
+// groups, so that each of its accesses is 1 KB (fp32) without a gap, and neighbouring lanes share their draws.  HBM-bound:
+// 65536 x 768 fp32 65 us, with a residual 97 us = 6.2 TB/s (a block a thread, two accesses 32 bytes apart: 73 and 105).
 template <class TX, class TY, bool RES, int MODE>
 __global__ __launch_bounds__(256) void dropout_add_wide_kernel(const TX* __restrict__ x, const TY* __restrict__ res,
                                                                unsigned blocks, Quotient per_row, Drop drop, Counter ctr,
@@ -116,7 +118,8 @@ __global__ __launch_bounds__(256) void dropout_add_short_kernel(const TX* __rest
     store_group(y + row * D, 0, D, v);
 }
 
-// part[slices][2][D] to the two gradients: 16 columns x 64 slice groups a workgroup, one tree over the groups -- a fixed order
+// part[slices][2][D] to the two gradients: 16 columns x 64 slice groups a workgroup, one tree over the groups -- a fixed order.
+// 3.9 us for 256 slices of 768 or 2048 columns, a launch and a read's latency (a thread a column over 512 slices: 118 us).
 __global__ __launch_bounds__(1024) void norm_param_reduce_kernel(const float* __restrict__ part, int slices, int D,
                                                                  void* __restrict__ grad_weight,
                                                                  void* __restrict__ grad_bias, int type) {

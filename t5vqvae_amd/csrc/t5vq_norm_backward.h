@@ -9,12 +9,15 @@ namespace t5vq_norm {
 //   grad_h = r (a - mean(a) - n mean(a n)) (+ g_sum), without mean(a) for rms;  grad_branch = kept ? grad_h * scale : 0;
 //   grad_weight = sum over rows of gy n, grad_bias = sum of gy.
 // The row stays in registers between its two sums and its gradients (group lane + G * j in chunk j, as forward), and a wave
-// adds up the parameters' gradients of all rows it walks: every input is read once.  Workgroup b leaves its sums in part[b].
+// adds up the parameters' gradients of all rows it walks: every input is read once.  Workgroup b leaves its sums in part[b];
+// one large workgroup a CU, so that these are few (4096 x 2048 bf16: 256 instead of 1024 slices 20.6 -> 17.4 us).
+// Bound by HBM in fp32 (65536 x 768 rms 99 us = 6.1 TB/s, with the sum's and the branch's gradients 171 us = 5.9 TB/s; keeping
+// a workgroup's waves in step past the caches 115 -> 104 and 194 -> 176 us a call); half rows of an odd length by the
+// vector pipe (33333 x 513 fp16 47 us for 171 MB: 500 instructions a row at three waves a SIMD).
 template <class TO, class TH, class TB, bool ADD, int G, int NCH, int WG, int MODE>
 __global__ __launch_bounds__(WG) void norm_backward_kernel(const TO* __restrict__ g, const TH* __restrict__ g_sum,
-                                                                     const TH* __restrict__ h, BackArgs a,
-                                                                     TH* __restrict__ grad_h, TB* __restrict__ grad_branch,
-                                                                     float* __restrict__ part) {
+                                                           const TH* __restrict__ h, BackArgs a, TH* __restrict__ grad_h,
+                                                           TB* __restrict__ grad_branch, float* __restrict__ part) {
     constexpr int ROWS = WG / G, SURE = sure<G, NCH, MODE>();
     __shared__ float slots[2][G > 64 ? ROWS : 1][G > 64 ? G / 64 : 1];
     __shared__ f32x4 sums[ROWS > 1 ? ROWS : 1][ROWS > 1 ? G * NCH : 1];
@@ -154,7 +157,8 @@ __global__ __launch_bounds__(WG) void norm_backward_kernel(const TO* __restrict_
     }
 }
 
-// Rows that registers do not hold (D > 8192), and rows shorter than one group (D < 4): one workgroup per row, read once for its sums and once for its gradients.
+// Rows that registers do not hold (D > 8192), and rows shorter than one group (D < 4): one workgroup per row, read once for its
+// sums and once for its gradients.  4096 x 20000 fp32 490 us = 2.0 TB/s.
 template <class TO, class TH, class TB>
 __global__ __launch_bounds__(256) void norm_backward_rows_kernel(const TO* __restrict__ g, const TH* __restrict__ g_sum,
                                                                  const TH* __restrict__ h, BackArgs a,
