@@ -68,7 +68,7 @@ class EncoderTailVQ(nn.Module):
         super().__init__()
         if dropout not in ("stored", "counter"):
             raise ValueError(f'dropout must be "stored" or "counter", got {dropout!r}')
-        if norm not in ops.NORM_KINDS:
+        if norm not in ("rms", "layer"):
             raise ValueError(f'norm must be "rms" or "layer", got {norm!r}')
         if dropout == "stored" and (norm != "rms" or branch_dropout_rate is not None or
                                     not (bias is None or bias is False)):
