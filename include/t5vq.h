@@ -463,7 +463,7 @@ int t5vq_norm_forward(const void* hidden, int hidden_type, const void* branch, i
  *   grad_branch = kept ? grad_hidden * scale : 0   (nullable; from grad_hidden before it is rounded)
  *   grad_weight[d] = sum_i gy n,  grad_bias[d] = sum_i gy   (nullable; of weight's type; deterministic, no atomics)
  * ticket: the forward's, null only if nothing was dropped.  Parameter gradients need a workspace of
- * t5vq_norm_backward_workspace_bytes(N, D) bytes. */
+ * t5vq_norm_backward_workspace_bytes(N, D) bytes (0 for few rows). */
 int64_t t5vq_norm_backward_workspace_bytes(int64_t N, int64_t D);
 int t5vq_norm_backward(const void* grad_out, int out_type, const void* grad_sum, const void* h, int hidden_type,
                        const void* weight, int weight_type, int norm_kind, const float* stats, int64_t N, int64_t D,

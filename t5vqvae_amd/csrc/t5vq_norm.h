@@ -372,8 +372,8 @@ struct BackArgs {
     void *grad_weight, *grad_bias;
 };
 
-// The norms of rows of one type (hidden); part: the parameters' sums or null; backward returns how many slices of them are
-// left to be added (0: the gradients are written already).
+// The norms of rows of one type (hidden); part: room for slices_of(N, D) slices of the parameters' sums (null without them);
+// backward returns how many are left to be added (0: the gradients are written already).
 #define T5VQ_NORM_TYPED(NAME)                                                                                              \
     void forward_##NAME(const void* hidden, const void* branch, int branch_type, void* out, int out_type, void* sum,       \
                         const NormArgs& a, hipStream_t stream);                                                            \
@@ -383,8 +383,11 @@ T5VQ_NORM_TYPED(f32)
 T5VQ_NORM_TYPED(bf16)
 T5VQ_NORM_TYPED(f16)
 #undef T5VQ_NORM_TYPED
-// How many workgroups share the rows of a backward call at most; each leaves 2 D floats of sums.
-inline int64_t slices_of(int64_t N) { return N < 2 * CUS ? N : 2 * CUS; }
+// How many workgroups share the rows of a backward call at most; each leaves 2 D floats of sums.  Up to four rows a wave (or
+// a workgroup, above 1024 columns) one takes them all and writes the gradients itself: its turns cost less than a second
+// launch (16 x 768: 12.4 -> 9.4 us a call).  ROWS of a workgroup are at least these (launch_back).
+inline int64_t rows_of_one(int64_t D) { return D < 4 || D > 8192 ? 0 : D <= 256 ? 128 : D <= 1024 ? 32 : D <= 4096 ? 8 : 4; }
+inline int64_t slices_of(int64_t N, int64_t D) { return N <= rows_of_one(D) ? 0 : N < 2 * CUS ? N : 2 * CUS; }
 
 inline bool known_type(int t) { return t == T5VQ_F32 || t == T5VQ_BF16 || t == T5VQ_F16; }
 inline int64_t type_bytes(int t) { return t == T5VQ_F32 ? 4 : 2; }

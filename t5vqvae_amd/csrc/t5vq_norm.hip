@@ -265,7 +265,7 @@ int t5vq_norm_forward(const void* hidden, int hidden_type, const void* branch, i
 }
 
 int64_t t5vq_norm_backward_workspace_bytes(int64_t N, int64_t D) {
-    return N > 0 && D > 0 ? slices_of(N) * 2 * D * 4 : 0;
+    return N > 0 && D > 0 ? slices_of(N, D) * 2 * D * 4 : 0;
 }
 
 int t5vq_norm_backward(const void* grad_out, int out_type, const void* grad_sum, const void* h, int hidden_type,
@@ -293,7 +293,8 @@ int t5vq_norm_backward(const void* grad_out, int out_type, const void* grad_sum,
                        (!grad_branch || (grad_branch != grad_out && grad_branch != grad_sum && grad_branch != h)),
                    "outputs must not be inputs, or each other");
     const bool params = grad_weight || grad_bias;
-    T5VQ_I_REQUIRE(!params || (workspace && workspace_bytes >= t5vq_norm_backward_workspace_bytes(N, D) &&
+    const int64_t room = params ? t5vq_norm_backward_workspace_bytes(N, D) : 0;
+    T5VQ_I_REQUIRE(!room || (workspace && workspace_bytes >= room &&
                                aligned_to(workspace, T5VQ_F32)),
                    "parameter gradients need a workspace of t5vq_norm_backward_workspace_bytes(N, D)");
     BackArgs a;
@@ -303,14 +304,14 @@ int t5vq_norm_backward(const void* grad_out, int out_type, const void* grad_sum,
     a.ctr = {0, 0, reinterpret_cast<const long long*>(ticket), ticket ? reinterpret_cast<const long long*>(ticket) + 1 : nullptr,
              nullptr};
     a.stats = stats, a.grad_weight = grad_weight, a.grad_bias = grad_bias;
-    float* part = params ? static_cast<float*>(workspace) : nullptr;
+    float* part = room ? static_cast<float*>(workspace) : nullptr;
     hipStream_t s = static_cast<hipStream_t>(stream);
     const int64_t slices = (hidden_type == T5VQ_F32    ? backward_f32
                             : hidden_type == T5VQ_BF16 ? backward_bf16
                                                        : backward_f16)(grad_out, out_type, grad_sum, h, a, grad_hidden,
                                                                        grad_branch, branch_type, part, s);
     T5VQ_I_CHECK_HIP(hipGetLastError());
-    if (params && slices) {
+    if (slices) {
         hipLaunchKernelGGL(norm_param_reduce_kernel, dim3(static_cast<unsigned>((D + 15) / 16), 2), dim3(1024), 0, s, part,
                            static_cast<int>(slices), a.D, grad_weight, grad_bias, weight_type);
         T5VQ_I_CHECK_HIP(hipGetLastError());

@@ -120,9 +120,9 @@ __global__ __launch_bounds__(WG) void norm_backward_kernel(const TO* __restrict_
         }
         if constexpr (TOGETHER) __syncthreads();   // the next row's sums reuse the slots
     }
-    if (!part) return;
+    if (!a.grad_weight && !a.grad_bias) return;
+    const bool only = !part;   // no other workgroup's sums to add: these are the gradients
     float* p = part + static_cast<size_t>(blockIdx.x) * 2 * D;
-    const bool only = gridDim.x == 1;   // no other workgroup's sums to add: these are the gradients
 #pragma unroll
     for (int j = 0; j < NCH; ++j) {
         gw[j] *= a.out.scale;
@@ -218,12 +218,12 @@ int64_t go(const void* g, const void* g_sum, const void* h, const BackArgs& a, v
            hipStream_t s) {
     constexpr auto kernel = norm_backward_kernel<TO, TH, TB, ADD, G, NCH, WG, MODE>;
     static const int64_t most = CUS * resident(kernel, WG);
-    // up to four rows a wave one workgroup takes them all: its turns cost less than a second launch
-    const int64_t wgs = a.N <= 4 * (WG / G) && part ? 1 : workgroups(a.N, WG / G, most < 2 * CUS ? most : 2 * CUS);
+    const bool params = a.grad_weight || a.grad_bias;
+    const int64_t wgs = params && !part ? 1 : workgroups(a.N, WG / G, most < 2 * CUS ? most : 2 * CUS);
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(wgs)), dim3(WG), 0, s, static_cast<const TO*>(g),
                        static_cast<const TH*>(g_sum), static_cast<const TH*>(h), a, static_cast<TH*>(grad_h),
                        static_cast<TB*>(grad_branch), part);
-    return wgs > 1 ? wgs : 0;
+    return part ? wgs : 0;
 }
 
 // ADD: with a gradient of the sum or for the branch.
@@ -258,7 +258,7 @@ int64_t launch_back(const void* g, const void* g_sum, const void* h, const BackA
                        dim3(256), 0, s, static_cast<const TO*>(g), static_cast<const TH*>(g_sum), static_cast<const TH*>(h), a,
                        static_cast<TH*>(grad_h), static_cast<TB*>(grad_branch));
     if (!part) return 0;
-    const int64_t slices = slices_of(a.N);
+    const int64_t slices = slices_of(a.N, a.D);
     hipLaunchKernelGGL((norm_param_grad_kernel<TO, TH>), dim3((a.D + 1023) / 1024, static_cast<unsigned>(slices)), dim3(256), 0,
                        s, static_cast<const TO*>(g), static_cast<const TH*>(h), a, part);
     return slices;

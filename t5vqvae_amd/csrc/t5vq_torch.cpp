@@ -495,7 +495,7 @@ std::tuple<Tensor, OptTensor, OptTensor, OptTensor> norm_backward(
     int64_t ws_bytes = 0;
     if (want_weight || want_bias) {
         ws_bytes = t5vq_norm_backward_workspace_bytes(N, D);
-        ws = at::empty({ws_bytes}, h.options().dtype(at::kByte));
+        if (ws_bytes) ws = at::empty({ws_bytes}, h.options().dtype(at::kByte));
     }
     ok(t5vq_norm_backward(g_out.data_ptr(), ot, ptr<void>(g_sum), h.data_ptr(), ht, weight.data_ptr(), wt,
                           static_cast<int>(kind), stats.data_ptr<float>(), N, D, branch_p, p, d.seed_dev, gh.data_ptr(),

@@ -24,36 +24,58 @@ from torch import nn
 from . import _lib, ops
 
 
-def _tensor(t, name):
-    if not isinstance(t, torch.Tensor):
-        raise TypeError(f"{name} must be a tensor")
-    return t
+_dropout = _norm = None          # torch.ops.t5vq's overloads, looked up once: these calls are short
+
+
+def _bind():
+    global _dropout, _norm
+    t5vq = _lib.load_torch_ops()
+    _dropout, _norm = t5vq.dropout.default, t5vq.norm.default
+
+
+def _not_a_tensor(name):
+    return TypeError(f"{name} must be a tensor")
 
 
 def dropout(x, p: float = 0.1, residual=None, *, training: bool = True, ticket=None):
     """``residual + dropout(x)`` (or ``dropout(x)``), of residual's type; ``training=False`` drops nothing."""
-    p = float(p) if training else 0.0
+    if not isinstance(x, torch.Tensor):
+        raise _not_a_tensor("x")
+    if not training:
+        p = 0.0
     if residual is None and ops.dropout_keep_count(p) == 65536:
-        return _tensor(x, "x")
-    return _lib.load_torch_ops().dropout.default(_tensor(x, "x"), residual, p, ticket)
+        return x
+    if _dropout is None:
+        _bind()
+    return _dropout(x, residual, p, ticket)
 
 
 def norm(hidden, weight, bias=None, *, kind: str = "layer", eps: float = 1e-6, p: float = 0.0, training: bool = True,
          ticket=None, out_dtype=None):
     """``dropout(norm(hidden) * weight + bias)``; ``kind``: "layer" (mean and variance) or "rms" (T5LayerNorm).
     ``out_dtype``: hidden's (default) or float32."""
-    return _lib.load_torch_ops().norm.default(_tensor(hidden, "hidden"), None, weight, bias, ops._norm_kind(kind), eps, 0.0,
-                                              p if training else 0.0, ticket, out_dtype)[0]
+    if not isinstance(hidden, torch.Tensor):
+        raise _not_a_tensor("hidden")
+    if kind not in ops.NORM_KINDS:
+        ops._norm_kind(kind)
+    if _norm is None:
+        _bind()
+    return _norm(hidden, None, weight, bias, ops.NORM_KINDS[kind], eps, 0.0, p if training else 0.0, ticket, out_dtype)[0]
 
 
 def add_norm(hidden, branch, weight, bias=None, *, kind: str = "layer", eps: float = 1e-6, branch_p: float = 0.0,
              p: float = 0.0, training: bool = True, ticket=None, out_dtype=None):
     """``(out, sum)``: sum = hidden + dropout(branch; branch_p) in hidden's type -- the residual stream that the next
     sublayer continues -- and out = dropout(norm(sum) * weight + bias; p)."""
+    if not (isinstance(hidden, torch.Tensor) and isinstance(branch, torch.Tensor)):
+        raise _not_a_tensor("hidden and branch")
     if not training:
         branch_p = p = 0.0
-    out, total = _lib.load_torch_ops().norm.default(_tensor(hidden, "hidden"), _tensor(branch, "branch"), weight, bias,
-                                                    ops._norm_kind(kind), eps, branch_p, p, ticket, out_dtype)
+    if kind not in ops.NORM_KINDS:
+        ops._norm_kind(kind)
+    if _norm is None:
+        _bind()
+    out, total = _norm(hidden, branch, weight, bias, ops.NORM_KINDS[kind], eps, branch_p, p, ticket, out_dtype)
     return out, total
 
 

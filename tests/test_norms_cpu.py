@@ -91,13 +91,13 @@ def test_c_abi_refuses_bad_calls_before_any_launch():
         return lib.t5vq_norm_backward(g, ot, gs, h, ht, w, wt, kind, st, n, d, bp, prob, ticket, gh, gb, bt, gw, gbias, ws,
                                       wsb, None)
 
-    need = lib.t5vq_norm_backward_workspace_bytes(4, 8)
-    assert need > 0 and lib.t5vq_norm_backward_workspace_bytes(0, 8) == 0
+    need = lib.t5vq_norm_backward_workspace_bytes(4000, 8)
+    assert need > 0 and lib.t5vq_norm_backward_workspace_bytes(0, 8) == 0 and lib.t5vq_norm_backward_workspace_bytes(4, 8) == 0
     for call in (dict(g=None), dict(h=None), dict(w=None), dict(st=None), dict(gh=None), dict(ot=BF16), dict(ht=9),
                  dict(ht=BF16, ot=BF16, gb=z_, bt=F32), dict(kind=-1), dict(n=0), dict(d=0), dict(prob=0.1),
-                 dict(gb=z_, bp=0.1), dict(gh=p), dict(gb=p), dict(gb=y_), dict(gs=y_), dict(prob=2.0, ticket=p), dict(gw=p), dict(gbias=p, ws=p, wsb=need - 1),
-                 dict(gw=p, ws=odd, wsb=need), dict(g=odd), dict(h=odd), dict(gs=odd), dict(gh=odd), dict(gb=odd),
-                 dict(gw=odd, ws=p, wsb=need)):
+                 dict(gb=z_, bp=0.1), dict(gh=p), dict(gb=p), dict(gb=y_), dict(gs=y_), dict(prob=2.0, ticket=p),
+                 dict(gw=p, n=4000), dict(gbias=p, ws=p, wsb=need - 1, n=4000), dict(gw=p, ws=odd, wsb=need, n=4000),
+                 dict(g=odd), dict(h=odd), dict(gs=odd), dict(gh=odd), dict(gb=odd), dict(gw=odd, ws=p, wsb=need)):
         assert back(**call) == 1, call
         assert lib.t5vq_last_error()
 
