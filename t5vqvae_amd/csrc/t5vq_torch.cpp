@@ -12,7 +12,9 @@
 #include <ATen/hip/HIPGeneratorImpl.h>
 #include <c10/core/DeviceGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/library.h>
 
 #include <mutex>
@@ -349,6 +351,9 @@ int need_param(const Tensor& t, const char* name, const Tensor& rows) {
                 rows.size(-1), " elements, got shape ", t.sizes());
     return type_of(t, name);
 }
+void need_kind(int64_t kind) {
+    TORCH_CHECK(kind == T5VQ_NORM_LAYER || kind == T5VQ_NORM_RMS, "kind must be 0 (layer) or 1 (rms), got ", kind);
+}
 
 // Where a forward call's random numbers come from: the caller's ticket, or the device's default generator of torch, which
 // is moved on by 8 (two sites of 4) under its lock -- inside a graph capture its state stays on the device and every replay
@@ -434,6 +439,7 @@ std::tuple<Tensor, OptTensor, OptTensor, OptTensor, OptTensor> norm_forward(
     const int bt = branch.has_value() ? need_rows(*branch, "branch", hidden) : ht;
     if (bias.has_value())
         TORCH_CHECK(need_param(*bias, "bias", hidden) == wt, "bias must be of weight's type, ", weight.scalar_type());
+    need_kind(kind);
     const int64_t N = rows_of(hidden), D = hidden.size(-1);
     if (token_image.has_value()) {
         TORCH_CHECK(need(*token_image, "token_image", at::kByte).numel() >= t5vq_token_image_bytes(N, D),
@@ -471,6 +477,7 @@ std::tuple<Tensor, OptTensor, OptTensor, OptTensor> norm_backward(
     const c10::DeviceGuard guard(h.device());
     const int ht = need_rows(h, "h", h), ot = need_rows(g_out, "g_out", h), wt = need_param(weight, "weight", h);
     if (g_sum.has_value()) TORCH_CHECK(need_rows(*g_sum, "g_sum", h) == ht, "g_sum must be of h's type, ", h.scalar_type());
+    need_kind(kind);
     const int64_t N = rows_of(h), D = h.size(-1);
     TORCH_CHECK(need(stats, "stats", at::kFloat, 2).size(0) == N && stats.size(1) == 2, "stats must be [", N, ", 2]");
     TORCH_CHECK(stats.device() == h.device(), "stats is on ", stats.device(), ", expected ", h.device());
@@ -525,6 +532,40 @@ variable_list once(variable_list grads) {
     return (*err)(std::move(grads));
 }
 
+// There is no forward-mode derivative either.
+void no_tangent(const Tensor& t) {
+    TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), "t5vq: dropout and norm have no forward-mode derivative");
+}
+void no_tangent(const OptTensor& t) {
+    if (t.has_value()) no_tangent(*t);
+}
+
+// A gradient accumulator lives as long as an eager graph of its leaf, on the stream that made it.  A captured backward pass
+// that hands it a gradient makes the default stream wait for the capture, which is not allowed and has ended processes:
+// refused while nothing of this node is recorded yet.
+void no_accumulator_outside_the_capture(const Tensor& g) {
+    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(static_cast<hipStream_t>(stream_of(g)), &capture) != hipSuccess) {
+        (void)hipGetLastError();   // the default stream beside another thread's capture: no capture of this one
+        return;
+    }
+    if (capture == hipStreamCaptureStatusNone) return;
+    const auto node = torch::autograd::get_current_node();
+    const auto* wanted = torch::autograd::get_current_graph_task_exec_info();
+    if (!node) return;
+    for (const auto& edge : node->next_edges()) {
+        if (!dynamic_cast<torch::autograd::AccumulateGrad*>(edge.function.get())) continue;
+        if (wanted && !wanted->empty()) {
+            const auto it = wanted->find(edge.function.get());
+            if (it == wanted->end() || !it->second.should_execute()) continue;
+        }
+        const auto stream = edge.function->stream();
+        TORCH_CHECK(!stream.has_value() || stream->id() != 0,
+                    "t5vq: this captured backward pass reaches a leaf whose gradient accumulator belongs to an eager graph on the "
+                    "default stream that still lives; free that graph (its outputs and losses) before the capture");
+    }
+}
+
 struct DropoutFunction : torch::autograd::Function<DropoutFunction> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& residual, double p, const OptTensor& ticket) {
         auto [y, drawn] = dropout_add(x.contiguous(), residual.has_value() ? OptTensor(residual->contiguous()) : residual, p,
@@ -536,6 +577,8 @@ struct DropoutFunction : torch::autograd::Function<DropoutFunction> {
         return y;
     }
     static variable_list backward(AutogradContext* ctx, variable_list g) {
+        no_tangent(g[0]);
+        no_accumulator_outside_the_capture(g[0]);
         const Tensor ticket = ctx->get_saved_variables()[0];
         variable_list out(4);
         if (ctx->needs_input_grad(0))
@@ -547,6 +590,8 @@ struct DropoutFunction : torch::autograd::Function<DropoutFunction> {
 };
 
 Tensor dropout_autograd(const Tensor& x, const OptTensor& residual, double p, const OptTensor& ticket) {
+    no_tangent(x);
+    no_tangent(residual);
     at::AutoDispatchBelowADInplaceOrView below;
     if (at::GradMode::is_enabled() && (asks(x) || asks(residual))) return DropoutFunction::apply(x, residual, p, ticket);
     return std::get<0>(
@@ -581,7 +626,9 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
         return norm_outputs(r);
     }
     static variable_list backward(AutogradContext* ctx, variable_list g) {
+        for (const auto& t : g) no_tangent(t);
         const auto saved = ctx->get_saved_variables();
+        no_accumulator_outside_the_capture(saved[0]);
         const Tensor &h = saved[0], &weight = saved[1], &stats = saved[2], &ticket = saved[3];
         const double branch_p = ctx->saved_data["branch_p"].toDouble();
         const bool branch = !ctx->saved_data["branch"].isNone();
@@ -613,6 +660,10 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
 variable_list norm_autograd(const Tensor& hidden, const OptTensor& branch, const Tensor& weight, const OptTensor& bias,
                             int64_t kind, double eps, double branch_p, double p, const OptTensor& ticket,
                             std::optional<at::ScalarType> out_dtype, bool row_norms, const OptTensor& token_image) {
+    no_tangent(hidden);
+    no_tangent(weight);
+    no_tangent(branch);
+    no_tangent(bias);
     at::AutoDispatchBelowADInplaceOrView below;
     if (at::GradMode::is_enabled() && (asks(hidden) || asks(branch) || asks(weight) || asks(bias)))
         return NormFunction::apply(hidden, branch, weight, bias, ticket, kind, eps, branch_p, p, out_dtype, row_norms,

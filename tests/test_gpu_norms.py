@@ -493,6 +493,20 @@ def test_refusals_on_the_device():
     (gx,) = torch.autograd.grad(y.sum(), x, create_graph=True)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(gx.sum(), x)
+    import torch.autograd.forward_ad as fwd
+    plain = torch.zeros(4, 16, device="cuda")
+    with fwd.dual_level():
+        dual = fwd.make_dual(plain, torch.ones_like(plain))
+        for call in (lambda: norms.dropout(dual, 0.1), lambda: norms.dropout(plain, 0.1, dual), lambda: norms.norm(dual, w),
+                     lambda: norms.norm(plain, fwd.make_dual(w, w)), lambda: norms.add_norm(plain, dual, w),
+                     lambda: torch.autograd.grad(y, x, dual, retain_graph=True)):
+            with pytest.raises(RuntimeError):
+                call()
+    for kind in (2, -1, 1 << 32):
+        with pytest.raises(RuntimeError):
+            torch.ops.t5vq.norm(plain, None, w, None, kind, EPS, 0.0, 0.0)
+        with pytest.raises(RuntimeError):
+            torch.ops.t5vq.norm_backward(plain, None, plain, w, st, kind, 0.0, 0.0, None, None, True, True)
 
 
 # ---- random numbers ---------------------------------------------------------------------------------------------------------
@@ -601,6 +615,70 @@ def test_first_call_of_a_kernel_inside_a_capture():
         check_backward(back, g, h, w, "rms", None, 0.0)
         keep = no.keep_mask(40, 5000, 0.5, drop[1].tolist(), 0)
         assert torch.equal(drop[0].cpu(), torch.where(keep, h.cpu() * 2, torch.zeros((), dtype=F16)))
+
+
+def test_captured_autograd_steps_follow_their_ticket():
+    """Forward and backward through autograd in one graph; the ticket's words change between replays."""
+    from t5vqvae_amd import norms
+    h, br, g, gs = (rows(200, 768, 211 + k).cuda() for k in range(4))
+    w, b = rows(1, 768, 215)[0].cuda(), rows(1, 768, 216)[0].cuda()
+    words = ticket()
+
+    def step():
+        x = [t.detach().requires_grad_(True) for t in (h, br, w, b)]
+        out, total = norms.add_norm(*x, eps=EPS, branch_p=0.1, p=0.1, ticket=words)
+        y = norms.dropout(out, 0.2, total, ticket=words)
+        return (y.detach(),) + torch.autograd.grad((y, total), x, (g, gs))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        res = step()
+    last = None
+    for k in range(4):
+        words.copy_(torch.tensor([77 + k, 8 * k]))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert last is None or not torch.equal(res[0], last)
+        last = res[0].clone()
+        for x, y in zip(res, step()):
+            assert torch.equal(x, y)
+
+
+def test_captured_backward_beside_a_living_eager_graph_is_refused():
+    """Leaves whose accumulators an eager graph on the default stream keeps: the capture's backward raises before it records
+    anything; once the eager graph is gone the same capture works."""
+    from t5vqvae_amd import norms
+    h, g = rows(50, 64, 221).cuda(), rows(50, 64, 222).cuda()
+    w = rows(1, 64, 223)[0].cuda().requires_grad_(True)
+    eager = norms.norm(h, w, eps=EPS)
+    (want,) = torch.autograd.grad(eager, w, g, retain_graph=True)
+    x, t = h.clone().requires_grad_(True), ticket()
+    dropped = norms.dropout(x, 0.5, ticket=t)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = h * 2.0                                           # the graph is not empty
+        out = norms.norm(h, w, eps=EPS)
+        with pytest.raises(RuntimeError, match="eager graph"):
+            torch.autograd.grad(out, w, g)
+        with pytest.raises(RuntimeError, match="eager graph"):
+            norms.dropout(x, 0.5, ticket=t).backward(g)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(held, h * 2.0) and x.grad is None and w.grad is None
+    del eager, dropped, out
+    again = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(again):
+        (got,) = torch.autograd.grad(norms.norm(h, w, eps=EPS), w, g)
+    for _ in range(3):
+        again.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
 
 
 def test_two_graphs_of_the_same_operators_replay_beside_each_other():
