@@ -379,6 +379,29 @@ def test_large_calls_equal_their_parts(n, d, dtype):
         check_backward((gh[part], gb[part], None, None), go[part], t[part], w, "rms", keep1, p, gs[part], keep0, p)
 
 
+@pytest.mark.parametrize("n,d", [(37, 768), (50, 64), (9, 2048), (3, 20000), (40, 2), (70000, 768)])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_views_that_start_at_any_element(n, d, dtype):
+    """Dense views one element behind an allocation's start (and parameters likewise) give what aligned copies give."""
+    from t5vqvae_amd import ops
+
+    def views(m, seed):
+        t = torch.randn(m * d + 1, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda").to(dtype)[1:]
+        t = t.view(m, d) if m > 1 else t
+        return t, t.clone()
+    h, br, g, gs, w, b = (views(m, 300 + i) for i, m in enumerate((n, n, n, n, 1, 1)))
+    res = []
+    for k in range(2):
+        y = ops.dropout_add(br[k], 0.3, h[k], ticket())[0]
+        only = ops.dropout_add(br[k], 0.3, None, ticket())[0]
+        out, total, stats, _, _ = ops.norm_forward(h[k], w[k], b[k], branch=br[k], branch_p=0.3, p=0.1, ticket=ticket())
+        res.append((y, only, out, total, stats) + tuple(
+            ops.norm_backward(g[k], gs[k], h[k], w[k], stats, branch_p=0.3, p=0.1, ticket=ticket(), branch_dtype=dtype)))
+    assert h[0].data_ptr() % 16 and not h[1].data_ptr() % 16
+    for x, y in zip(*res):
+        assert torch.equal(x, y)
+
+
 # ---- outputs for the searches --------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("n,d", [(1, 64), (45, 768), (130, 2048), (33, 100), (257, 1024), (64, 1536), (31, 192), (50, 256), (7, 140),
                                  (9, 300), (12, 512), (5, 640)])
