@@ -297,9 +297,10 @@ struct Place {
     }
 };
 // Chunks that are whole in every row a kernel of G lanes and NCH chunks is called for (launch_norm, launch_back): all of them
-// where D = 4 G NCH, all but the last else -- but for four chunks of 256 lanes or more, which start at half.
+// where D = 4 G NCH, all but the last else -- but for four chunks of 256 lanes, which start at half, and
+// six and eight of 512, at two less.
 template <int G, int NCH, int MODE>
-constexpr int sure() { return MODE != RAGGED ? NCH : NCH == 4 && G >= 256 ? 2 : NCH - 1; }
+constexpr int sure() { return MODE != RAGGED ? NCH : (NCH == 4 && G == 256) || NCH > 4 ? NCH - 2 : NCH - 1; }
 
 // sum over the G lanes of a row (16, or a multiple of 64), fixed order; slots: G / 64 floats of LDS a row, and one more set for
 // the next call, which may then write before every wave has read this one's
@@ -386,7 +387,7 @@ T5VQ_NORM_TYPED(f16)
 // How many workgroups share the rows of a backward call at most; each leaves 2 D floats of sums.  Up to four rows a wave (or
 // a workgroup, above 1024 columns) one takes them all and writes the gradients itself: its turns cost less than a second
 // launch (16 x 768: 12.4 -> 9.4 us a call).  ROWS of a workgroup are at least these (launch_back).
-inline int64_t rows_of_one(int64_t D) { return D < 4 || D > 8192 ? 0 : D <= 256 ? 128 : D <= 1024 ? 32 : D <= 4096 ? 8 : 4; }
+inline int64_t rows_of_one(int64_t D) { return D < 4 || D > 16384 ? 0 : D <= 256 ? 128 : D <= 1024 ? 32 : D <= 4096 ? 8 : 4; }
 inline int64_t slices_of(int64_t N, int64_t D) { return N <= rows_of_one(D) ? 0 : N < 2 * CUS ? N : 2 * CUS; }
 
 inline bool known_type(int t) { return t == T5VQ_F32 || t == T5VQ_BF16 || t == T5VQ_F16; }

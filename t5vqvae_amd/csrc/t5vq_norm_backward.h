@@ -13,7 +13,9 @@ namespace t5vq_norm {
 // one large workgroup a CU, so that these are few (4096 x 2048 bf16: 256 instead of 1024 slices 20.6 -> 17.4 us).
 // Bound by HBM in fp32 (65536 x 768 rms 99 us = 6.1 TB/s, with the sum's and the branch's gradients 171 us = 5.9 TB/s; keeping
 // a workgroup's waves in step past the caches 115 -> 104 and 194 -> 176 us a call); half rows of an odd length by the
-// vector pipe (33333 x 513 fp16 47 us for 171 MB: 500 instructions a row at three waves a SIMD).
+// vector pipe (33333 x 513 fp16 47 us for 171 MB: 500 instructions a row at three waves a SIMD).  Rows past 8192 columns are
+// read without a next one in flight, at half the waves and twice the chunks of a 1024-thread workgroup, which spilled (8192 x
+// 12288 bf16 139 us = 4.3 TB/s, three passes over memory 348 us; x 16384 177 us, with sum and branch it spills: 270 us).
 template <class TO, class TH, class TB, bool ADD, int G, int NCH, int WG, int MODE>
 __global__ __launch_bounds__(WG) void norm_backward_kernel(const TO* __restrict__ g, const TH* __restrict__ g_sum,
                                                            const TH* __restrict__ h, BackArgs a, TH* __restrict__ grad_h,
@@ -23,6 +25,7 @@ __global__ __launch_bounds__(WG) void norm_backward_kernel(const TO* __restrict_
     __shared__ f32x4 sums[ROWS > 1 ? ROWS : 1][ROWS > 1 ? G * NCH : 1];
     // a workgroup's waves keep step where they share a row, and past the caches, where rows that are read together lie together
     constexpr bool TOGETHER = G > 64 || MODE == STREAMED;
+    constexpr bool AHEAD = NCH <= 4;   // the next row is on its way while one is worked on: not where registers hold one alone
     const Place<G, WG> at;
     const unsigned lane = at.lane, D = MODE != RAGGED ? 4 * G * NCH : a.D;
     const Key k0 = site_key(a.ctr, 0), k1 = site_key(a.ctr, 1);
@@ -46,7 +49,7 @@ __global__ __launch_bounds__(WG) void norm_backward_kernel(const TO* __restrict_
             vn[j] = load_at<SURE, MODE>(j, g + t * D, 4 * (lane + G * j), D);
             nn[j] = load_at<SURE, MODE>(j, h + t * D, 4 * (lane + G * j), D);
         }
-        if (ADD && g_sum) {
+        if (ADD && AHEAD && g_sum) {
 #pragma unroll
             for (int j = 0; j < (ADD ? NCH : 0); ++j) sn[j] = load_at<SURE, MODE>(j, g_sum + t * D, 4 * (lane + G * j), D);
         }
@@ -56,22 +59,23 @@ __global__ __launch_bounds__(WG) void norm_backward_kernel(const TO* __restrict_
     const bool drops = ADD && grad_branch && a.branch.kept < 65536u, drops_out = a.out.kept < 65536u;
     Bits last0 = {0, 0}, last1 = {0, 0};   // of the last of an odd number of chunks, where a draw gave it in advance
     bool ahead = false;
-    if (first + at.sub < a.N) fetch(first + at.sub);
+    if (AHEAD && first + at.sub < a.N) fetch(first + at.sub);
     for (long long base = first; base < a.N; base += step) {
         const long long row = base + at.sub;
         // where waves wait for each other every one of them comes along, with a row of its own or without
         const bool live = row < a.N;
         if (!TOGETHER && !live) break;
+        if (!AHEAD) fetch(row);
         f32x4 v[NCH], n[NCH];
         typename Group<TH>::type gs[ADD ? NCH : 1];
 #pragma unroll
         for (int j = 0; j < NCH; ++j) {
             v[j] = live ? widen_at<SURE>(j, vn[j], 4 * (lane + G * j), D) : zero4;
             n[j] = live ? widen_at<SURE>(j, nn[j], 4 * (lane + G * j), D) : zero4;
-            if constexpr (ADD) gs[j] = sn[j];
+            if constexpr (ADD && AHEAD) gs[j] = sn[j];
         }
         const float mean = mean_n, r = r_n;
-        if (row + step < a.N) fetch(row + step);
+        if (AHEAD && row + step < a.N) fetch(row + step);
         const unsigned r32 = static_cast<unsigned>(row);
         Bits bits = {0, 0};
         if constexpr (NCH & 1) {
@@ -100,6 +104,10 @@ __global__ __launch_bounds__(WG) void norm_backward_kernel(const TO* __restrict_
             s2 = fmaf(v[j].y, n[j].y, s2);
             s2 = fmaf(v[j].z, n[j].z, s2);
             s2 = fmaf(v[j].w, n[j].w, s2);
+        }
+        if (ADD && !AHEAD && g_sum) {
+#pragma unroll
+            for (int j = 0; j < (ADD ? NCH : 0); ++j) gs[j] = load_at<SURE, MODE>(j, g_sum + row * D, 4 * (lane + G * j), D);
         }
         s1 = a.layer ? row_sum<G>(s1, slots[0][G > 64 ? at.sub : 0], lane) * inv_d : 0.f;
         s2 = row_sum<G>(s2, slots[1][G > 64 ? at.sub : 0], lane) * inv_d;
@@ -157,7 +165,7 @@ __global__ __launch_bounds__(WG) void norm_backward_kernel(const TO* __restrict_
     }
 }
 
-// Rows that registers do not hold (D > 8192), and rows shorter than one group (D < 4): one workgroup per row, read once for its
+// Rows that registers do not hold (D > 16384), and rows shorter than one group (D < 4): one workgroup per row, read once for its
 // sums and once for its gradients.  4096 x 20000 fp32 490 us = 2.0 TB/s.
 template <class TO, class TH, class TB>
 __global__ __launch_bounds__(256) void norm_backward_rows_kernel(const TO* __restrict__ g, const TH* __restrict__ g_sum,
@@ -242,7 +250,7 @@ int64_t launch_back(const void* g, const void* g_sum, const void* h, const BackA
                : bytes < STREAM_BYTES ? go<TO, TH, TB, ADD, G, NCH, T, WHOLE>(g, g_sum, h, a, grad_h, grad_branch, part, s)  \
                                       : go<TO, TH, TB, ADD, G, NCH, T, STREAMED>(g, g_sum, h, a, grad_h, grad_branch, part, s); \
     } while (0)
-    if (a.D >= 4 && a.D <= 8192) {
+    if (a.D >= 4 && a.D <= 16384) {
         if (a.D <= 64) T5VQ_NBK(16, 1, 768, 768, 768);
         if (a.D <= 128) T5VQ_NBK(16, 2, 768, 768, 768);
         if (a.D <= 192) T5VQ_NBK(16, 3, 768, 768, 768);
@@ -252,7 +260,10 @@ int64_t launch_back(const void* g, const void* g_sum, const void* h, const BackA
         if (a.D <= 1024) T5VQ_NBK(64, 4, 512, 768, 768);
         if (a.D <= 2048) T5VQ_NBK(256, 2, 1024, 1024, 1024);
         if (a.D <= 4096) T5VQ_NBK(256, 4, 512, 768, 512);
-        return go<TO, TH, TB, ADD, 1024, 2, 1024, RAGGED>(g, g_sum, h, a, grad_h, grad_branch, part, s);
+        if (a.D <= 6144) T5VQ_NBK(512, 3, 512, 512, 512);
+        if (a.D <= 8192) T5VQ_NBK(512, 4, 512, 512, 512);
+        if (a.D <= 12288) return go<TO, TH, TB, ADD, 512, 6, 512, RAGGED>(g, g_sum, h, a, grad_h, grad_branch, part, s);
+        return go<TO, TH, TB, ADD, 512, 8, 512, RAGGED>(g, g_sum, h, a, grad_h, grad_branch, part, s);
     }
 #undef T5VQ_NBK
     hipLaunchKernelGGL((norm_backward_rows_kernel<TO, TH, TB>), dim3(static_cast<unsigned>(workgroups(a.N, 1, CUS * 8))),

@@ -16,6 +16,8 @@ namespace t5vq_norm {
 // Bound by HBM in fp32 (65536 x 768: norm 69 us = 5.8 TB/s, add + norm 140 us = 5.8 TB/s), by HBM and the vector pipe alike in
 // half types with a dropout (bf16: norm 38.7 us = 5.2 TB/s, 27.5 us of issue, two thirds of them draws).  16 lanes a row
 // instead of 64: 65536 x 192 bf16 19.5 -> 12.6 us, x 64 69 -> 16 us.  2880 x 768 fp32 7.1 us, one row 2.4 us: latency.
+// 512 lanes a row up to 8192 columns instead of 1024: two rows a CU take turns at their barriers, and 5120 columns fill five
+// sixths of the lanes' chunks (16384 x 5120 bf16 97 -> 68 us, x 8192 100 -> 91 us = 5.9 TB/s).
 template <class TH, class TB, class TO, bool ADD, int G, int NCH, int MODE>
 __global__ __launch_bounds__(G > 256 ? G : 256) void norm_kernel(const TH* __restrict__ hidden, const TB* __restrict__ branch,
                                                                  TO* __restrict__ out, TH* __restrict__ sum, NormArgs a) {
@@ -230,7 +232,9 @@ void launch_norm(const void* hidden, const void* branch, void* out, void* sum, c
     else if (a.D <= 1024) T5VQ_NK(64, 4);
     else if (a.D <= 2048) T5VQ_NK(256, 2);
     else if (a.D <= 4096) T5VQ_NK(256, 4);
-    else if (a.D <= 8192) go<TH, TB, TO, ADD, 1024, 2, RAGGED>(hidden, branch, out, sum, a, stream);
+    else if (a.D <= 6144) T5VQ_NK(512, 3);
+    else if (a.D <= 8192) T5VQ_NK(512, 4);
+    else if (a.D <= 12288) go<TH, TB, TO, ADD, 1024, 3, RAGGED>(hidden, branch, out, sum, a, stream);
     else go<TH, TB, TO, ADD, 1024, 4, RAGGED>(hidden, branch, out, sum, a, stream);
 #undef T5VQ_NK
 }

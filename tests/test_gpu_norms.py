@@ -338,8 +338,31 @@ def test_gradients_are_the_slopes_of_the_forward(kind):
         assert abs(got - slope) <= 1e-5 * size, (i, got, slope)
 
 
+@pytest.mark.parametrize("n,d", [(5, 4097), (3, 5120), (9, 6144), (4, 6145), (300, 8192), (5, 8193), (4, 10241), (600, 12288),
+                                 (5, 12289), (7, 16383), (6, 16384), (3, 16385)])
+@pytest.mark.parametrize("hidden,branch,out,wdtype,kind", [
+    (F32, F32, F32, F32, "layer"), (F32, BF16, F32, F32, "rms"), (BF16, BF16, BF16, BF16, "layer"), (F16, F16, F32, F32, "rms")])
+def test_long_rows(n, d, hidden, branch, out, wdtype, kind):
+    """Where a row's lanes and chunks change, up to where registers do not hold it: both norms forward and backward."""
+    from t5vqvae_amd import ops
+    p, bp = 0.2, 0.3
+    h, br, w, b = rows(n, d, 401, hidden), rows(n, d, 402, branch), rows(1, d, 403, wdtype)[0], rows(1, d, 404, wdtype)[0]
+    g, gs = rows(n, d, 405, out).cuda(), rows(n, d, 406, hidden).cuda()
+    keep0, keep1 = no.keep_mask(n, d, bp, TICKET, 0), no.keep_mask(n, d, p, TICKET, 1)
+    y, total, stats, _, _ = ops.norm_forward(h.cuda(), w.cuda(), b.cuda(), kind=kind, eps=EPS, branch=br.cuda(), branch_p=bp,
+                                             p=p, ticket=ticket(), out_dtype=out)
+    assert torch.equal(total, ops.dropout_add(br.cuda(), bp, h.cuda(), ticket())[0])
+    check_forward(y, total, w, b, kind, keep1, p, out)
+    plain = ops.norm_forward(total, w.cuda(), b.cuda(), kind=kind, eps=EPS, p=p, ticket=ticket(), out_dtype=out)
+    assert torch.equal(plain[0], y) and torch.equal(plain[2], stats)
+    got = ops.norm_backward(g, gs, total, w.cuda(), stats, kind=kind, branch_p=bp, p=p, ticket=ticket(), branch_dtype=branch)
+    check_backward(got, g, total, w, kind, keep1, p, gs, keep0, bp)
+    got = ops.norm_backward(g, None, total, w.cuda(), stats, kind=kind, p=p, ticket=ticket())
+    check_backward(got, g, total, w, kind, keep1, p)
+
+
 @pytest.mark.parametrize("n,d,dtype", [(65541, 768, F32), (131083, 768, BF16), (800005, 64, F32), (50003, 1024, F16),
-                                       (25003, 2048, F32)])
+                                       (25003, 2048, F32), (10003, 6144, F32), (7003, 8192, F32)])
 def test_large_calls_equal_their_parts(n, d, dtype):
     """Calls that go past the caches (192 MB and more) against the same rows in small calls, bit for bit, and the oracle's
     masks on the last rows; the parameters' gradients against float64 sums."""
