@@ -339,11 +339,12 @@ def test_gradients_are_the_slopes_of_the_forward(kind):
 
 
 @pytest.mark.parametrize("n,d", [(5, 4097), (3, 5120), (9, 6144), (4, 6145), (300, 8192), (5, 8193), (4, 10241), (600, 12288),
-                                 (5, 12289), (7, 16383), (6, 16384), (3, 16385)])
+                                 (5, 12289), (7, 16383), (6, 16384), (3, 16385), (70001, 3), (1030, 2), (300, 1)])
 @pytest.mark.parametrize("hidden,branch,out,wdtype,kind", [
     (F32, F32, F32, F32, "layer"), (F32, BF16, F32, F32, "rms"), (BF16, BF16, BF16, BF16, "layer"), (F16, F16, F32, F32, "rms")])
-def test_long_rows(n, d, hidden, branch, out, wdtype, kind):
-    """Where a row's lanes and chunks change, up to where registers do not hold it: both norms forward and backward."""
+def test_long_and_short_rows(n, d, hidden, branch, out, wdtype, kind):
+    """Where a row's lanes and chunks change, up to where registers do not hold it, and rows of less than one group: both
+    norms forward and backward."""
     from t5vqvae_amd import ops
     p, bp = 0.2, 0.3
     h, br, w, b = rows(n, d, 401, hidden), rows(n, d, 402, branch), rows(1, d, 403, wdtype)[0], rows(1, d, 404, wdtype)[0]
