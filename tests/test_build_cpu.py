@@ -77,3 +77,12 @@ def test_objects_follow_the_makefile(tree):
     makefile.write_text(makefile.read_text().replace("-O3", "-O2"))
     compiled, linked = tree()
     assert set(compiled) == sources(tree) and all("-O2" in line for line in compiled.values()) and len(linked) == 1
+
+
+def test_build_compiles_also_where_a_built_library_is_there(monkeypatch):
+    import __graft_entry__ as entry
+    calls = []
+    monkeypatch.setattr(entry.subprocess, "run", lambda args, **kw: calls.append((args, kw)))
+    entry.build()
+    (args, kw), = calls
+    assert args[0] == "make" and "-B" in args and "all" in args and kw == {"check": True}
