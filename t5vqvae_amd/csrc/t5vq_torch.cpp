@@ -512,9 +512,28 @@ std::tuple<Tensor, OptTensor, OptTensor, OptTensor> norm_backward(
     return {gh, gb, gw, gbias};
 }
 
-// ---- the same with a gradient (t5vqvae_amd.norms): one dispatcher crossing forward, none of Python's backward ------------
+// ---- the same with a gradient (t5vqvae_amd.norms): nothing of Python's, forward or backward --------------------------------
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
+
+// Autograd calls the operators above through the dispatcher, so that modes (fake tensors, loggers) see them: a fake tensor is
+// refused by its own mode before a generator has moved on.
+template <class F>
+c10::TypedOperatorHandle<F> registered(const char* name, F&) {
+    return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
+}
+#define T5VQ_THROUGH_DISPATCHER(name)                                     \
+    template <class... A>                                                  \
+    auto call_##name(A&&... a) {                                           \
+        static const auto op = registered("t5vq::" #name, name);           \
+        at::AutoDispatchBelowADInplaceOrView below;                        \
+        return op.call(std::forward<A>(a)...);                             \
+    }
+T5VQ_THROUGH_DISPATCHER(dropout_add)
+T5VQ_THROUGH_DISPATCHER(dropout_backward)
+T5VQ_THROUGH_DISPATCHER(norm_forward)
+T5VQ_THROUGH_DISPATCHER(norm_backward)
+#undef T5VQ_THROUGH_DISPATCHER
 
 OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
 Tensor bare(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
@@ -568,8 +587,8 @@ void no_accumulator_outside_the_capture(const Tensor& g) {
 
 struct DropoutFunction : torch::autograd::Function<DropoutFunction> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& residual, double p, const OptTensor& ticket) {
-        auto [y, drawn] = dropout_add(x.contiguous(), residual.has_value() ? OptTensor(residual->contiguous()) : residual, p,
-                                      ticket);
+        auto [y, drawn] = call_dropout_add(x.contiguous(),
+                                           residual.has_value() ? OptTensor(residual->contiguous()) : residual, p, ticket);
         ctx->save_for_backward({ticket.has_value() ? *ticket : bare(drawn)});
         ctx->saved_data["p"] = p;
         ctx->saved_data["type"] = x.scalar_type();
@@ -582,8 +601,8 @@ struct DropoutFunction : torch::autograd::Function<DropoutFunction> {
         const Tensor ticket = ctx->get_saved_variables()[0];
         variable_list out(4);
         if (ctx->needs_input_grad(0))
-            out[0] = dropout_backward(g[0].contiguous(), ctx->saved_data["p"].toDouble(), opt(ticket),
-                                      ctx->saved_data["type"].toScalarType());
+            out[0] = call_dropout_backward(g[0].contiguous(), ctx->saved_data["p"].toDouble(), opt(ticket),
+                                           ctx->saved_data["type"].toScalarType());
         if (ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(1)) out[1] = g[0];
         return once(std::move(out));
     }
@@ -595,7 +614,7 @@ Tensor dropout_autograd(const Tensor& x, const OptTensor& residual, double p, co
     at::AutoDispatchBelowADInplaceOrView below;
     if (at::GradMode::is_enabled() && (asks(x) || asks(residual))) return DropoutFunction::apply(x, residual, p, ticket);
     return std::get<0>(
-        dropout_add(x.contiguous(), residual.has_value() ? OptTensor(residual->contiguous()) : residual, p, ticket));
+        call_dropout_add(x.contiguous(), residual.has_value() ? OptTensor(residual->contiguous()) : residual, p, ticket));
 }
 
 // outputs of a norm as one list: out, sum with a branch, row norms on request
@@ -612,8 +631,8 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
                                  double p, std::optional<at::ScalarType> out_dtype, bool row_norms,
                                  const OptTensor& token_image) {
         const Tensor h = hidden.contiguous();
-        const auto r = norm_forward(h, branch.has_value() ? OptTensor(branch->contiguous()) : branch, weight, bias, kind, eps,
-                                    branch_p, p, ticket, out_dtype, true, row_norms, token_image);
+        const auto r = call_norm_forward(h, branch.has_value() ? OptTensor(branch->contiguous()) : branch, weight, bias, kind,
+                                         eps, branch_p, p, ticket, out_dtype, true, row_norms, token_image);
         ctx->save_for_backward({branch.has_value() ? *std::get<1>(r) : h, weight, *std::get<2>(r),
                                 ticket.has_value() ? *ticket : bare(std::get<4>(r))});
         ctx->saved_data["kind"] = kind;
@@ -640,15 +659,15 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
         variable_list out(12);
         if (!g[0].defined()) {                       // nothing came back through the norm: the sum's gradient only
             if (ctx->needs_input_grad(0)) out[0] = g_sum;
-            if (need_branch && g_sum.defined()) out[1] = dropout_backward(g_sum, branch_p, opt(ticket), branch_type);
+            if (need_branch && g_sum.defined()) out[1] = call_dropout_backward(g_sum, branch_p, opt(ticket), branch_type);
             return once(std::move(out));
         }
         // without a dropout of the branch its gradient is the stream's, unless it is of another type
         const bool same = branch_type == h.scalar_type() && !drops(branch_p, "branch_p");
-        const auto r = norm_backward(g[0].contiguous(), opt(g_sum), h, weight, stats, ctx->saved_data["kind"].toInt(), branch_p,
-                                     ctx->saved_data["p"].toDouble(), opt(ticket),
-                                     need_branch && !same ? std::optional<at::ScalarType>(branch_type) : std::nullopt,
-                                     need_weight, need_bias);
+        const auto r = call_norm_backward(g[0].contiguous(), opt(g_sum), h, weight, stats, ctx->saved_data["kind"].toInt(),
+                                          branch_p, ctx->saved_data["p"].toDouble(), opt(ticket),
+                                          need_branch && !same ? std::optional<at::ScalarType>(branch_type) : std::nullopt,
+                                          need_weight, need_bias);
         if (ctx->needs_input_grad(0)) out[0] = std::get<0>(r);
         if (need_branch) out[1] = same ? std::get<0>(r) : *std::get<1>(r);
         out[2] = bare(std::get<2>(r));
@@ -668,8 +687,9 @@ variable_list norm_autograd(const Tensor& hidden, const OptTensor& branch, const
     if (at::GradMode::is_enabled() && (asks(hidden) || asks(branch) || asks(weight) || asks(bias)))
         return NormFunction::apply(hidden, branch, weight, bias, ticket, kind, eps, branch_p, p, out_dtype, row_norms,
                                    token_image);
-    return norm_outputs(norm_forward(hidden.contiguous(), branch.has_value() ? OptTensor(branch->contiguous()) : branch, weight,
-                                     bias, kind, eps, branch_p, p, ticket, out_dtype, false, row_norms, token_image));
+    return norm_outputs(call_norm_forward(hidden.contiguous(), branch.has_value() ? OptTensor(branch->contiguous()) : branch,
+                                          weight, bias, kind, eps, branch_p, p, ticket, out_dtype, false, row_norms,
+                                          token_image));
 }
 
 // Tensors that are not on a ROCm device: there is no CPU path, say so instead of the dispatcher's listing

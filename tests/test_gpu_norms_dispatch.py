@@ -1,0 +1,65 @@
+"""Dropout and the norms under torch's dispatch modes on the device: what the modes see, that results do not depend on them,
+and that a refused call leaves the generator where it was."""
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode, UnsupportedOperatorException
+from torch.utils._python_dispatch import TorchDispatchMode
+
+pytestmark = pytest.mark.gpu
+
+
+class Log(TorchDispatchMode):
+    def __init__(self):
+        super().__init__()
+        self.names = []
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        if func.namespace == "t5vq":
+            self.names.append(func._opname)
+        return func(*args, **(kwargs or {}))
+
+
+def tensors(n=37, d=96):
+    g = torch.Generator(device="cuda").manual_seed(501)
+    h, br, go, gs = (torch.randn(n, d, generator=g, device="cuda") for _ in range(4))
+    w, b = torch.randn(d, generator=g, device="cuda"), torch.randn(d, generator=g, device="cuda")
+    return h, br, w, b, go, gs
+
+
+def step(h, br, w, b, go, gs):
+    from t5vqvae_amd import norms
+    leaves = [t.detach().requires_grad_(True) for t in (h, br, w, b)]
+    out, total = norms.add_norm(*leaves, branch_p=0.2, p=0.1)
+    y = norms.dropout(out, 0.3, total)
+    return (y.detach(), total.detach()) + torch.autograd.grad((y, total), leaves, (go, gs))
+
+
+def test_a_mode_sees_the_operators_and_changes_nothing():
+    from t5vqvae_amd import norms
+    x = tensors()
+    torch.manual_seed(7)
+    plain = step(*x)
+    torch.manual_seed(7)
+    with Log() as log:
+        seen = step(*x)
+    assert log.names == ["norm_forward", "dropout_add", "dropout_backward", "norm_backward"]
+    assert all(torch.equal(a, b) for a, b in zip(plain, seen))
+    with torch.no_grad(), Log() as log:
+        norms.norm(x[0], x[2])
+        norms.dropout(x[0], 0.5)
+    assert log.names == ["norm_forward", "dropout_add"]
+
+
+def test_fake_tensors_leave_the_generator_alone():
+    from t5vqvae_amd import norms
+    torch.manual_seed(3)
+    state = torch.cuda.get_rng_state()
+    for grad in (False, True):
+        with FakeTensorMode():
+            x = torch.empty(4, 8, device="cuda", requires_grad=grad)
+            w = torch.empty(8, device="cuda", requires_grad=grad)
+            for call in (lambda: norms.dropout(x, 0.5), lambda: norms.norm(x, w, p=0.5),
+                         lambda: norms.add_norm(x, x, w, branch_p=0.5)):
+                with pytest.raises(UnsupportedOperatorException):
+                    call()
+    assert torch.equal(torch.cuda.get_rng_state(), state)
