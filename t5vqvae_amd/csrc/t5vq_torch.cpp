@@ -14,6 +14,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/graph_task.h>
 #include <torch/library.h>
 
@@ -540,15 +541,27 @@ Tensor bare(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
 bool asks(const Tensor& t) { return t.defined() && t.requires_grad(); }
 bool asks(const OptTensor& t) { return t.has_value() && asks(*t); }
 
-// The gradients that a backward pass gives, for a pass that itself records a graph (create_graph): they look differentiable,
-// and differentiating them is refused -- there is no second derivative here, and none is silently taken as zero.
-variable_list once(variable_list grads) {
-    if (!at::GradMode::is_enabled()) return grads;
-    for (auto& g : grads)
-        if (g.defined()) g = g.detach().requires_grad_(true);
-    auto err = std::make_shared<torch::autograd::DelayedError>("t5vq: gradients of dropout and norm cannot be differentiated again",
-                                                               static_cast<int64_t>(grads.size()));
-    return (*err)(std::move(grads));
+// There is no second derivative here, and none is silently taken as zero: in a pass that itself records a graph
+// (create_graph) a gradient that was computed depends on what the call's gradients were made from -- the gradients that came
+// in and the running node's first `inputs` inputs -- through a node that refuses.  (Edges that lead nowhere would let a
+// derivative by those inputs pass this gradient by.)
+template <size_t M>
+void once(std::initializer_list<Tensor*> grads, const Tensor (&incoming)[M], size_t inputs) {
+    if (!at::GradMode::is_enabled()) return;
+    torch::autograd::edge_list from;
+    for (const auto& t : incoming)
+        if (t.defined() && t.requires_grad()) from.push_back(torch::autograd::impl::gradient_edge(t));
+    if (const auto node = torch::autograd::get_current_node())
+        for (size_t i = 0; i < inputs && i < node->num_outputs(); ++i)
+            if (node->next_edge(i).is_valid()) from.push_back(node->next_edge(i));
+    if (from.empty()) return;
+    const auto refuse = std::make_shared<torch::autograd::Error>("t5vq: gradients of dropout and norm cannot be differentiated again",
+                                                                 std::move(from));
+    for (Tensor* g : grads)
+        if (g->defined()) {
+            *g = g->detach();
+            torch::autograd::set_history(*g, refuse);
+        }
 }
 
 // There is no forward-mode derivative either.
@@ -603,8 +616,9 @@ struct DropoutFunction : torch::autograd::Function<DropoutFunction> {
         if (ctx->needs_input_grad(0))
             out[0] = call_dropout_backward(g[0].contiguous(), ctx->saved_data["p"].toDouble(), opt(ticket),
                                            ctx->saved_data["type"].toScalarType());
+        once({&out[0]}, {g[0]}, 0);               // linear in g: not a function of the inputs
         if (ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(1)) out[1] = g[0];
-        return once(std::move(out));
+        return out;
     }
 };
 
@@ -660,7 +674,8 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
         if (!g[0].defined()) {                       // nothing came back through the norm: the sum's gradient only
             if (ctx->needs_input_grad(0)) out[0] = g_sum;
             if (need_branch && g_sum.defined()) out[1] = call_dropout_backward(g_sum, branch_p, opt(ticket), branch_type);
-            return once(std::move(out));
+            once({&out[1]}, {g_sum}, 0);
+            return out;
         }
         // without a dropout of the branch its gradient is the stream's, unless it is of another type
         const bool same = branch_type == h.scalar_type() && !drops(branch_p, "branch_p");
@@ -672,7 +687,8 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
         if (need_branch) out[1] = same ? std::get<0>(r) : *std::get<1>(r);
         out[2] = bare(std::get<2>(r));
         out[3] = bare(std::get<3>(r));
-        return once(std::move(out));
+        once({&out[0], &out[1], &out[2], &out[3]}, {g[0], g_sum}, branch ? 3 : 2);   // of hidden, branch and weight
+        return out;
     }
 };
 
