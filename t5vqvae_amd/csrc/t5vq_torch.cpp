@@ -12,7 +12,6 @@
 #include <ATen/hip/HIPGeneratorImpl.h>
 #include <c10/core/DeviceGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/graph_task.h>
@@ -23,6 +22,7 @@
 #include <tuple>
 
 #include "t5vq.h"
+#include "t5vq_graph_walk.h"
 
 namespace {
 
@@ -572,10 +572,12 @@ void no_tangent(const OptTensor& t) {
     if (t.has_value()) no_tangent(*t);
 }
 
-// A gradient accumulator lives as long as an eager graph of its leaf, on the stream that made it.  A captured backward pass
-// that hands it a gradient makes the default stream wait for the capture, which is not allowed and has ended processes:
-// refused while nothing of this node is recorded yet.
-void no_accumulator_outside_the_capture(const Tensor& g) {
+// A node of an autograd graph belongs to the stream that made it; a leaf's accumulator is such a node, and lives as long as any
+// graph of the leaf does.  A captured backward pass that hands a gradient to a node of the default stream makes that stream wait
+// for the capture, which is not allowed and has ended processes: refused while nothing of the running node is recorded yet, if
+// the pass would reach such a node behind it, be it through casts, views or other operations.  (What it reaches by other ways
+// only is not seen here.)
+void no_eager_graph_behind_the_capture(const Tensor& g) {
     hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
     if (hipStreamIsCapturing(static_cast<hipStream_t>(stream_of(g)), &capture) != hipSuccess) {
         (void)hipGetLastError();   // the default stream beside another thread's capture: no capture of this one
@@ -583,19 +585,23 @@ void no_accumulator_outside_the_capture(const Tensor& g) {
     }
     if (capture == hipStreamCaptureStatusNone) return;
     const auto node = torch::autograd::get_current_node();
-    const auto* wanted = torch::autograd::get_current_graph_task_exec_info();
     if (!node) return;
-    for (const auto& edge : node->next_edges()) {
-        if (!dynamic_cast<torch::autograd::AccumulateGrad*>(edge.function.get())) continue;
-        if (wanted && !wanted->empty()) {
-            const auto it = wanted->find(edge.function.get());
-            if (it == wanted->end() || !it->second.should_execute()) continue;
-        }
-        const auto stream = edge.function->stream();
-        TORCH_CHECK(!stream.has_value() || stream->id() != 0,
-                    "t5vq: this captured backward pass reaches a leaf whose gradient accumulator belongs to an eager graph on the "
-                    "default stream that still lives; free that graph (its outputs and losses) before the capture");
-    }
+    using torch::autograd::Node;
+    const auto* wanted = torch::autograd::get_current_graph_task_exec_info();   // empty: everything runs
+    const bool all = !wanted || wanted->empty();
+    const auto runs = [&](Node* n) {
+        if (all) return true;
+        const auto it = wanted->find(n);
+        return it != wanted->end() && it->second.should_execute();
+    };
+    const auto eager = [](Node* n) {
+        const auto stream = n->stream();
+        return stream.has_value() && stream->id() == 0;
+    };
+    TORCH_CHECK(!t5vq_graph::first_behind(*node, runs, eager),
+                "t5vq: this captured backward pass reaches an eager graph on the default stream -- a leaf whose gradient accumulator "
+                "such a graph keeps, or one of its operations; free that graph (its outputs and losses) before the capture, or make "
+                "it inside");
 }
 
 struct DropoutFunction : torch::autograd::Function<DropoutFunction> {
@@ -610,7 +616,7 @@ struct DropoutFunction : torch::autograd::Function<DropoutFunction> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list g) {
         no_tangent(g[0]);
-        no_accumulator_outside_the_capture(g[0]);
+        no_eager_graph_behind_the_capture(g[0]);
         const Tensor ticket = ctx->get_saved_variables()[0];
         variable_list out(4);
         if (ctx->needs_input_grad(0))
@@ -661,7 +667,7 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
     static variable_list backward(AutogradContext* ctx, variable_list g) {
         for (const auto& t : g) no_tangent(t);
         const auto saved = ctx->get_saved_variables();
-        no_accumulator_outside_the_capture(saved[0]);
+        no_eager_graph_behind_the_capture(saved[0]);
         const Tensor &h = saved[0], &weight = saved[1], &stats = saved[2], &ticket = saved[3];
         const double branch_p = ctx->saved_data["branch_p"].toDouble();
         const bool branch = !ctx->saved_data["branch"].isNone();
