@@ -80,20 +80,20 @@ __device__ __forceinline__ void store_at(int j, T* __restrict__ row, unsigned c,
 }
 // Reads of the other chunks do not branch (a branch would wait for every read already on its way): a group that reaches past
 // the row's end, or lies behind it, reads the row's last four elements (D >= 4), and widen_at puts them in their places
-// when they are there, 0 behind the end.
+// when they are there, `fill` behind the end.
 template <int SURE, int MODE = WHOLE, class T>
 __device__ __forceinline__ typename Group<T>::type load_at(int j, const T* __restrict__ row, unsigned c, unsigned D) {
     const unsigned at = (j < SURE || c + 4 <= D ? c : D - 4) * static_cast<unsigned>(sizeof(T));
     return read<MODE>(reinterpret_cast<const typename Group<T>::type*>(reinterpret_cast<const char*>(row) + at));
 }
 template <int SURE, class V>
-__device__ __forceinline__ f32x4 widen_at(int j, V raw, unsigned c, unsigned D) {
-    const f32x4 v = widen(raw), zero = {0.f, 0.f, 0.f, 0.f};
+__device__ __forceinline__ f32x4 widen_at(int j, V raw, unsigned c, unsigned D, float fill = 0.f) {
+    const f32x4 v = widen(raw), all = {fill, fill, fill, fill};
     if (j < SURE) return v;
     const unsigned behind = (0u - D) & 3u;   // how many of the last group's columns do not exist: the same for the whole call
-    const f32x4 last = {behind == 1 ? v.y : behind == 2 ? v.z : v.w, behind == 1 ? v.z : behind == 2 ? v.w : 0.f,
-                        behind == 1 ? v.w : 0.f, 0.f};
-    return c + 4 <= D ? v : (c < D ? last : zero);
+    const f32x4 last = {behind == 1 ? v.y : behind == 2 ? v.z : v.w, behind == 1 ? v.z : behind == 2 ? v.w : fill,
+                        behind == 1 ? v.w : fill, fill};
+    return c + 4 <= D ? v : (c < D ? last : all);
 }
 // a block's two groups, read as load_at reads them, and one of them widened (FROM: 0 or 4)
 template <class T>

@@ -68,13 +68,14 @@ __global__ __launch_bounds__(WG) void norm_backward_kernel(const TO* __restrict_
         if (!AHEAD) fetch(row);
         f32x4 v[NCH], n[NCH];
         typename Group<TH>::type gs[ADD ? NCH : 1];
+        // where no column is, g is 0 and h the mean, so that n is 0 as well: mean * r may be infinite
+        const float mean = live ? mean_n : 0.f, r = r_n;
 #pragma unroll
         for (int j = 0; j < NCH; ++j) {
             v[j] = live ? widen_at<SURE>(j, vn[j], 4 * (lane + G * j), D) : zero4;
-            n[j] = live ? widen_at<SURE>(j, nn[j], 4 * (lane + G * j), D) : zero4;
+            n[j] = live ? widen_at<SURE>(j, nn[j], 4 * (lane + G * j), D, mean) : zero4;
             if constexpr (ADD && AHEAD) gs[j] = sn[j];
         }
-        const float mean = mean_n, r = r_n;
         if (AHEAD && row + step < a.N) fetch(row + step);
         const unsigned r32 = static_cast<unsigned>(row);
         Bits bits = {0, 0};
@@ -95,7 +96,7 @@ __global__ __launch_bounds__(WG) void norm_backward_kernel(const TO* __restrict_
         float s1 = 0.f, s2 = 0.f;
 #pragma unroll
         for (int j = 0; j < NCH; ++j) {
-            n[j] = (n[j] - mean) * r;      // behind the row's end g is 0: what n is there reaches no sum
+            n[j] = (n[j] - mean) * r;
             gw[j] = fma4(v[j], n[j], gw[j]);
             gb[j] += v[j];
             v[j] *= w[j];
@@ -223,7 +224,7 @@ __global__ __launch_bounds__(256) void norm_backward_rows_kernel(const TO* __res
         };
         float s1 = 0.f, s2 = 0.f;
         for (int q = tid; q < groups; q += 256) {
-            const f32x4 v = upstream(q), n = (load_group(h + row * D, 4 * q, D) - mean) * r;
+            const f32x4 v = upstream(q), n = inside((load_group(h + row * D, 4 * q, D) - mean) * r, 4 * q, D);
             s1 = sum4(v, s1);
             s2 = sum4(v * n, s2);
         }
