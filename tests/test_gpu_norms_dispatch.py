@@ -63,3 +63,26 @@ def test_fake_tensors_leave_the_generator_alone():
                 with pytest.raises(UnsupportedOperatorException):
                     call()
     assert torch.equal(torch.cuda.get_rng_state(), state)
+
+
+def test_tensors_that_stand_for_their_negative():
+    """A view whose negation torch has put off (the imaginary part of a conjugate) is negated before a kernel reads it: rows,
+    parameters and incoming gradients."""
+    from t5vqvae_amd import norms
+    h, br, w, b, go, gs = tensors()
+    t = torch.tensor([3, 8], device="cuda")
+
+    def run(view):
+        leaves = [v.detach().requires_grad_(True) for v in (h, br, w, b)]
+        x = [view(v) for v in leaves]
+        out, total = norms.add_norm(*x, branch_p=0.2, p=0.1, ticket=t)
+        y = norms.dropout(x[0], 0.3, out, ticket=t)
+        plain = norms.norm(x[1], x[2], x[3])
+        with torch.no_grad():
+            quiet = norms.norm(x[0], x[2], x[3], p=0.1, ticket=t)
+        grads = torch.autograd.grad((y, total, plain), leaves, (view(go), view(gs), view(go)))
+        return (y.detach(), total.detach(), plain.detach(), quiet) + grads
+    lazy, done = run(torch._neg_view), run(torch.neg)
+    assert torch._neg_view(h).is_neg()
+    for a, c in zip(lazy, done):
+        assert torch.equal(a, c)
