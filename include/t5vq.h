@@ -413,14 +413,15 @@ int t5vq_rmsnorm_sqnorms_img_f32(const float* hidden, const float* gamma, const 
 
 /* ---- Dropout from a counter, layer / RMS norm, and the sum of a residual stream with a sublayer's output ----------
  * What stands around the encoder's last norm: the dropout and residual sum of the sublayer before it, the norm, and the
- * dropout behind it (python_transformers/modeling_t5.py:864-865), for fp32, bf16 and fp16 rows of any length D >= 1 that start at any multiple of their element's size.  Arithmetic, statistics and
- * sums are fp32; every output is rounded once, to nearest even.
+ * dropout behind it (python_transformers/modeling_t5.py:864-865), for fp32, bf16 and fp16 rows of any length D >= 1 that start
+ * at any multiple of their element's size.  Arithmetic, statistics and sums are fp32; every output is rounded once, to nearest
+ * even.
  *
  * Random numbers.  No mask is stored: a kernel draws an element's 16 bits from Philox4x32-10 (Salmon et al., SC 2011)
  * with the key `seed` and the counter (offset / 4 + site: 64 bits, col / 8: 32 bits, row: 32 bits); column 8b + j takes
  * half j % 2 (low half first) of word j / 2.  It is kept iff those bits are below K = t5vq_dropout_keep_count(p) =
  * round_half_even((1 - p) * 65536), and a kept value is multiplied by fp32(65536 / K), so the expectation is exact
- * although p is rounded to a multiple of 2^-16.  A dropped value is 0 whatever it was.  K == 65536 (p < 2^-17): no
+ * although p is rounded to a multiple of 2^-16.  A dropped value is 0 whatever it was.  K == 65536 (p <= 2^-17): no
  * dropout; K == 0: everything is dropped.
  *   Forward calls take {seed, offset} by value, and (both nullable) from device memory: *seed_dev REPLACES seed,
  *   *offset_dev is ADDED to offset -- a generator that a graph replays, or an earlier call's ticket.  ticket_out

@@ -23,6 +23,9 @@ enum { RAGGED, WHOLE, STREAMED };
 // Measured with every call's output kept (us; in brackets the call and a kernel that reads its output): 65536 x 768 bf16 norm,
 // 201 MB, 42.2 -> 39.8 (75.9 -> 71.4), its backward, 302 MB, 65.5 -> 59.6 (101 -> 91); 65536 x 768 fp32 norm 80 -> 74;
 // 16384 x 768 fp32 norm, 101 MB, 23.4 -> 21.0 (37.2 -> 39.0): below, the neighbour loses what it would find in the cache.
+// With outputs freed at once, at 64 to 6144 columns: 100 MB 19-24 -> 23-30, 252 MB (bf16 norm) 43-51 -> 47-54 and (bf16 add + norm
+// backward) 46-54 -> 50-57, 302 MB (fp32 norm backward) 57-68 -> 55-66, 378 MB (bf16) 74-84 -> 67-79, 503 MB (fp32 norm) 96-100 ->
+// 86-88, (fp32 add + norm backward) 100-108 -> 87-95, 1259 MB 245-261 -> 216-230: such a caller gains from 300 MB on.
 constexpr int64_t STREAM_BYTES = 192ll << 20;
 
 // eight elements: a Philox block's columns
@@ -182,7 +185,8 @@ struct Words { unsigned w0, w1, w2, w3; };
 // (site offset, block of eight columns, row): words 0, 1 belong to the block's lower group of four, 2, 3 to its upper one,
 // 16 bits an element, low half first.  Any lane can draw any element's bits at any time: the mask is never stored.  A draw is
 // 20 products of 32 x 32 -> 64 bits (v_mad_u64_u32; 15 where the offset and the row are the wave's) and 20 three-way xors,
-// about 110 instructions with its exchange for the 8 elements of two lanes' groups.
+// about 110 instructions with its exchange for the 8 elements of two lanes' groups.  Alone on a SIMD a wave's product takes 2.3 ns, a
+// three-way xor 1.8, a fused multiply-add of fp32 1.1.
 __device__ __forceinline__ Words philox(const Key k, unsigned block, unsigned row) {
     unsigned a = k.c0, b = k.c1, c = block, d = row, k0 = k.k0, k1 = k.k1;
 #pragma unroll
@@ -384,9 +388,11 @@ T5VQ_NORM_TYPED(f32)
 T5VQ_NORM_TYPED(bf16)
 T5VQ_NORM_TYPED(f16)
 #undef T5VQ_NORM_TYPED
-// How many workgroups share the rows of a backward call at most; each leaves 2 D floats of sums.  Up to four rows a wave (or
-// a workgroup, above 1024 columns) one takes them all and writes the gradients itself: its turns cost less than a second
-// launch (16 x 768: 12.4 -> 9.4 us a call).  ROWS of a workgroup are at least these (launch_back).
+// How many workgroups share the rows of a backward call at most; each leaves 2 D floats of sums.  Up to these rows one takes them
+// all, in four turns at most -- ROWS of a workgroup are 32 or more, 8, 2 and 1 (launch_back) --, and writes the gradients itself: go()
+// launches exactly one where part is null.  Measured with a workgroup's slices and the second launch against this, us a call: 16 x 768
+// 12.5 -> 8.0, 128 x 64 12.5 -> 8.0, 128 x 256 12.5 -> 9.0, 32 x 1024 12.5 -> 8.0, 8 x 4096 12.3 -> 10.4, 4 x 8192 12.3 -> 9.9,
+// 2 x 16384 13.4 -> 11.0; above 8192 columns the last rows lose (3 x 16384 13.5 -> 14.2, 4 x 8200 12.5 -> 14.2, 4 x 16384 13.6 -> 17.3).
 inline int64_t rows_of_one(int64_t D) { return D < 4 || D > 16384 ? 0 : D <= 256 ? 128 : D <= 1024 ? 32 : D <= 4096 ? 8 : 4; }
 inline int64_t slices_of(int64_t N, int64_t D) { return N <= rows_of_one(D) ? 0 : N < 2 * CUS ? N : 2 * CUS; }
 

@@ -10,8 +10,8 @@ namespace {
 
 // y = residual + (kept ? x * scale : 0).  A thread takes U blocks of eight columns, 256 blocks apart, so that each Philox block
 // is drawn once and U blocks of every input are on their way together.  WHOLE: D % 8 == 0, rows follow each other without
-// a gap and a block of a half type is one access of 16 bytes.  HBM-bound: 65536 x 768 bf16 with a residual 48 us = 6.3 TB/s, of
-// which the draws' issue fills 21; rows of 513 fp16 16.9 -> 18.9 us with them.
+// a gap and a block of a half type is one access of 16 bytes.  HBM-bound: 65536 x 768 bf16 with a residual 48 us = 6.3 TB/s, 47 us
+// without the draws; rows of 513 fp16 16.9 -> 18.9 us with them.
 template <class TX, class TY, bool RES, int MODE>
 __global__ __launch_bounds__(256) void dropout_add_kernel(const TX* __restrict__ x, const TY* __restrict__ res, unsigned D,
                                                           unsigned blocks, Quotient per_row, Drop drop, Counter ctr,
@@ -68,7 +68,8 @@ __global__ __launch_bounds__(256) void dropout_add_kernel(const TX* __restrict__
 
 // The same for whole blocks with fp32 on either side, where a block is two accesses: a wave takes 64 blocks as two times 64
 // groups, so that each of its accesses is 1 KB (fp32) without a gap, and neighbouring lanes share their draws.  HBM-bound:
-// 65536 x 768 fp32 65 us, with a residual 97 us = 6.2 TB/s (a block a thread, two accesses 32 bytes apart: 73 and 105).
+// 65536 x 768 fp32 65 us, with a residual 97 us = 6.2 TB/s (a block a thread, two accesses 32 bytes apart: 73 and 105); a bf16 or
+// fp16 branch into an fp32 stream 83 us = 6.1 TB/s.
 template <class TX, class TY, bool RES, int MODE>
 __global__ __launch_bounds__(256) void dropout_add_wide_kernel(const TX* __restrict__ x, const TY* __restrict__ res,
                                                                unsigned blocks, Quotient per_row, Drop drop, Counter ctr,

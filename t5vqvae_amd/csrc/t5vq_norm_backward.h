@@ -12,8 +12,9 @@ namespace t5vq_norm {
 // adds up the parameters' gradients of all rows it walks: every input is read once.  Workgroup b leaves its sums in part[b];
 // one large workgroup a CU, so that these are few (4096 x 2048 bf16: 256 instead of 1024 slices 20.6 -> 17.4 us).
 // Bound by HBM in fp32 (65536 x 768 rms 99 us = 6.1 TB/s, with the sum's and the branch's gradients 171 us = 5.9 TB/s; keeping
-// a workgroup's waves in step past the caches 115 -> 104 and 194 -> 176 us a call); half rows of an odd length by the
-// vector pipe (33333 x 513 fp16 47 us for 171 MB: 500 instructions a row at three waves a SIMD).  Rows past 8192 columns are
+// a workgroup's waves in step past the caches 115 -> 104 and 194 -> 176 us a call; a bf16 or fp16 branch beside an fp32 stream 151 us =
+// 6.0 TB/s, bf16 rows with an fp32 output 102 us = 5.9 TB/s); half rows of an odd length by their instructions (33333 x 513 fp16 47 us
+// for 171 MB: 500 a row at three waves a SIMD; 4 us less without the draws).  Rows past 8192 columns are
 // read without a next one in flight, at half the waves and twice the chunks of a 1024-thread workgroup, which spilled (8192 x
 // 12288 bf16 139 us = 4.3 TB/s, three passes over memory 348 us; x 16384 177 us, with sum and branch it spills: 270 us).
 template <class TO, class TH, class TB, bool ADD, int G, int NCH, int WG, int MODE>
@@ -281,9 +282,11 @@ int64_t launch_back(const void* g, const void* g_sum, const void* h, const BackA
                     float* part, hipStream_t s) {
     const int64_t bytes = a.N * a.D * static_cast<int64_t>(sizeof(TO) + 2 * sizeof(TH) + (g_sum ? sizeof(TH) : 0) +
                                                            (grad_branch ? sizeof(TB) : 0));
-// One workgroup fills a CU with the waves that its registers leave room for (occupancy 2 .. 4 of a SIMD's 512 registers), so
-// that few workgroups leave sums behind: WG threads, and for whole rows of a plain norm W (half types) or P (fp32).  (A sum or a
-// branch at W: 65536 x 768 bf16 with an fp32 output spilled, 158 us against 105; 32768 x 4096 bf16 235 against 225 us.)
+// One large workgroup a CU (two to four waves a SIMD), so that few workgroups leave sums behind: WG threads, and for whole rows of a
+// plain norm W (half types) or P (fp32).  (A sum or a branch at W: 65536 x 768 bf16 with an fp32 output spilled, 158 us against 105;
+// 32768 x 4096 bf16 235 against 225 us.)  The sizes do not follow the registers everywhere: up to 2048 columns the bf16 norm takes 72, which
+// would leave room for seven waves a SIMD where there are four; fp32 rows with a sum or a branch spill at 768 threads on 16 x 3 (28
+// bytes a lane, streamed 12) and ragged 64 x 3 (28), and 512 x 8 spills with a sum or a branch (fp32 440 to 488, half types 156 to 228).
 #define T5VQ_NBK(G, NCH, WG, W, P)                                                                                           \
     do {                                                                                                                     \
         constexpr int T = ADD ? WG : sizeof(TH) == 2 ? W : P;                                                                \

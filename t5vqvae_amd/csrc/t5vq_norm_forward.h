@@ -13,8 +13,10 @@ namespace t5vq_norm {
 // A row in registers: G lanes hold it, group lane + G * j in chunk j of NCH.  One read of each input, one write of each
 // output; G = 16 (four rows a wave) or 64 (one) without a barrier, a workgroup a row above.  The parameters stay in registers
 // while a wave walks its rows, and the next row is on its way while this one is worked on.
-// Bound by HBM in fp32 (65536 x 768: norm 69 us = 5.8 TB/s, add + norm 140 us = 5.8 TB/s), by HBM and the vector pipe alike in
-// half types with a dropout (bf16: norm 38.7 us = 5.2 TB/s, 27.5 us of issue, two thirds of them draws).  16 lanes a row
+// Bound by HBM in fp32 (65536 x 768: norm 69 us = 5.8 TB/s, add + norm 140 us = 5.8 TB/s), and in half types but for what the
+// draws add (bf16: norm 39 us = 5.2 TB/s, 37.8 without its dropout; with an fp32 output 55.5 us = 5.4 TB/s).  Ragged rows add the work on
+// lane places that hold nothing, and never go past the caches (bf16, 50 M elements: 896 columns 38 us, 640 41, 1536 and 2560 53,
+// 1280 64; fp32 76 to 82).  16 lanes a row
 // instead of 64: 65536 x 192 bf16 19.5 -> 12.6 us, x 64 69 -> 16 us.  2880 x 768 fp32 7.1 us, one row 2.4 us: latency.
 // 512 lanes a row up to 8192 columns instead of 1024: two rows a CU take turns at their barriers, and 5120 columns fill five
 // sixths of the lanes' chunks (16384 x 5120 bf16 97 -> 68 us, x 8192 100 -> 91 us = 5.9 TB/s).
