@@ -204,7 +204,7 @@ int t5vq_cosine_backward_f32(const float* x, const float* q, const float* g_out,
                              t5vq_stream_t stream);
 
 /* enc[N,K] = one-hot(idx) in fp32 (vqvae/vqvae.py:124-125).  Off the hot path: every caller of the
- * reference discards it (SURVEY.md 8b). */
+ * reference discards it. */
 int t5vq_one_hot_f32(const int64_t* idx, int64_t N, int64_t K, float* enc, t5vq_stream_t stream);
 
 /* ---- The same search, filtered in fp16 and decided in fp32 (no reference counterpart: an implementation choice) --
@@ -232,7 +232,7 @@ int t5vq_dist_argmin_filtered_f32(const float* x, const float* w, float* xx, flo
                                   int64_t code_offset, int exact_keys, void* workspace, int64_t workspace_bytes,
                                   int64_t* keys, int32_t* n_overflow, t5vq_stream_t stream);
 
-/* ---- Evaluation-side searches (callers of the path in evaluate_vqvae.py; SURVEY.md 8f rank 3) ----------------
+/* ---- Evaluation-side searches (callers of the path in evaluate_vqvae.py) ----------------
  *
  * The topk nearest codes per token in ascending (distance, index) order -- what
  *   a, idx1 = torch.sort(distances[dim]); idx = idx1[:top_k]          (evaluate_vqvae.py:129-135)
@@ -249,7 +249,7 @@ int t5vq_dist_topk_f32(const float* x, const float* w, const float* xx, const fl
 int t5vq_blend_argmin_f32(const float* dist_left, const float* dist_right, float weight_left, float weight_right,
                           int64_t N, int64_t K, int64_t* keys, t5vq_stream_t stream);
 
-/* ---- Encoder tail fused into the VQ prologue (SURVEY.md 8f rank 2) ------------------------------------------
+/* ---- Encoder tail fused into the VQ prologue ------------------------------------------
  *
  * T5LayerNorm (python_transformers/modeling_t5.py:191-207: no mean subtraction, learned scale) followed by dropout
  * (:864-865, and :853-854 at the mid-encoder call site) produce the tensor the VQ receives (t5/load_t5.py:518).
@@ -271,7 +271,7 @@ int t5vq_rmsnorm_backward_f32(const float* grad_x, const float* hidden, const fl
                               float scale, const float* rms, int64_t N, int64_t D, float* grad_hidden,
                               float* grad_gamma, float* workspace, t5vq_stream_t stream);
 
-/* ---- Composite calls: what a replacement of the module's forward must export (SURVEY.md 8b) ------------------
+/* ---- Composite calls: what a replacement of the module's forward must export ------------------
  * They chain the entry points above on `stream`; results are bit-identical to calling them one by one.
  *
  * t5vq_vq_forward_f32 = vqvae/vqvae.py:103-128,147-152,160 (plain variant :24-64,71) plus the EMA statistics

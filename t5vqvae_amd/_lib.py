@@ -89,8 +89,8 @@ TORCH_LIB_PATH = os.environ.get("T5VQ_TORCH_LIB") or os.path.join(_HERE, "csrc",
 _lib = None
 _torch_ops = None
 # A failed load is remembered and re-raised: a second ``dlopen`` / ``torch.ops.load_library`` of a library whose first
-# load threw half-way (its static registrations partly run) is undefined -- in round 2 such a retry, made by the autograd
-# worker thread of a backward-only flow, hung inside ``run_backward`` (DESIGN.md section 11).
+# load threw half-way (its static registrations partly run) is undefined: such a retry, made by the autograd
+# worker thread of a backward-only flow, hung inside ``run_backward``.
 _lib_error = None
 _torch_ops_error = None
 

@@ -7,7 +7,7 @@
 //
 //   d(i,k)   = fl(fl(xx_i + ee_k) - 2 dot(i,k)),  dot = the k-ordered fp32 fma chain of the scan kernel
 //   d~(i,k)  = the same expression with dot~ = fp16(x_i) . fp16(e_k) (rows scaled by powers of two) accumulated in fp32 by the MFMA
-//   |d~ - d| <= delta(i,k) = c2 |x_i| |e_k| + r (xx_i + ee_k)          (bound derived in DESIGN.md section 8)
+//   |d~ - d| <= delta(i,k) = c2 |x_i| |e_k| + r (xx_i + ee_k)          (bound derived where c2 is computed)
 //   T_i = min_k (d~ + delta)                     >= d(i, k*) for the true argmin k*
 //   candidates {k : d~ - delta <= T_i}           contain k* and every code tied with it
 //   refine: exact d for the candidates in the scan kernel's summation order, packed-key minimum
@@ -906,7 +906,7 @@ int t5vq_internal_dist_argmin_filtered(const float* x, const float* w, float* xx
     }
     T5VQ_I_CHECK_HIP(hipGetLastError());
 
-    // error coefficient of the fp16 dot product against the fp32 chain, relative to |x| |e| (DESIGN.md section 8):
+    // error coefficient of the fp16 dot product against the fp32 chain, relative to |x| |e|:
     // two operand roundings (u = 2^-11 each; elements below 2^-28 of their row maximum fall into fp16's denormals:
     // absolute error 2^-39 of the maximum when rounded, 2^-28 if the pipe flushed them to zero -- the sqrt(D) 2^-26
     // term covers both operands either way), the matrix pipe's fp32 accumulation of the exact

@@ -1600,7 +1600,7 @@ __global__ __launch_bounds__(256) void ema_embed_kernel(float* __restrict__ ema_
 }
 
 // ------------------------------------------------------------------------------------------------
-// Encoder tail fused into the VQ prologue (SURVEY 8f rank 2): T5LayerNorm (RMS norm, no mean subtraction, learned
+// Encoder tail fused into the VQ prologue: T5LayerNorm (RMS norm, no mean subtraction, learned
 // scale) + dropout produce the VQ input; the same pass also emits the row norms |x|^2 the distance kernel needs.
 // One wave per row; lane layout as everywhere: float4 #(j*64 + lane).
 // ------------------------------------------------------------------------------------------------

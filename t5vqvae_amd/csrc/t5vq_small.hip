@@ -1,4 +1,4 @@
-// t5vq_small.hip -- the single-launch forward for SMALL problems (BASELINE config 2: N = 4096, K = 512, D = 768).
+// t5vq_small.hip -- the single-launch forward for SMALL problems (N = 4096, K = 512, D = 768).
 //
 // At this size a launch costs as much as the work it carries: the chain [distance + argmin] -> [gather + statistics] ->
 // [scalars] ran 35 + 11 + 4 us against 20.5 us of matrix work.  Here ONE kernel does the whole forward of

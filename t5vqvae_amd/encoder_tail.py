@@ -1,4 +1,4 @@
-"""Encoder tail fused into the VQ prologue (SURVEY.md 8f rank 2).
+"""Encoder tail fused into the VQ prologue.
 
 In the reference the tensor the VQ receives is ``dropout(final_layer_norm(hidden_states))``
 (python_transformers/modeling_t5.py:864-865, consumed at t5/load_t5.py:518; the mid-encoder call site applies the
@@ -9,7 +9,7 @@ result once more just to form |x|^2.  ``EncoderTailVQ`` does norm + dropout + |x
 returns the gradients of the hidden states and of the norm weight.
 
 A maintainer who wants the fusion replaces ``final_layer_norm`` / ``dropout`` of the encoder stack by identities
-and calls this module where ``self.vqvae(encoding, srl_ids)`` is called (INTEGRATION.md section 4).  The plain
+and calls this module where ``self.vqvae(encoding, srl_ids)`` is called.  The plain
 drop-in (``VectorQuantizerEMA`` alone) does not need it.
 
 The dropout mask is drawn with torch's generator (``bernoulli_``) and passed to the kernel as a uint8 tensor, or

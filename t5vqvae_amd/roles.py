@@ -1,5 +1,5 @@
 """Host side of the disentangled (role-grouped) codebook: per-token code ranges as the reference's loader builds
-them, and the index convention the quantizer applies to them (SURVEY.md 8f rank 4).
+them, and the index convention the quantizer applies to them.
 
 The reference stores one ``(start, end)`` pair per token in ``batch['srl']`` (t5/load_data.py:68-99): every word's
 semantic-role label is looked up in ``dimension_dict`` (e.g. ``{"V": (0, 1000), "residual": (1000, K)}``,

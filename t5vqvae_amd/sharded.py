@@ -1,14 +1,14 @@
 """Multi-GPU forms of the VQ bottleneck: one process per GPU, torch.distributed (backend "nccl" = RCCL
 over xGMI on ROCm; "gloo" in the CPU tests of the host logic).
 
-Token sharding -- ``shard_tokens(module)``.
+Token sharding (N = 2^20 tokens over 8 GPUs) -- ``shard_tokens(module)``.
     Every rank holds N/G tokens and a full replica of the codebook state.  Distances, argmin, gather and the
     loss terms are per token, so the only exchange is ONE all-reduce(sum) of the fused statistics buffer
     [embed_sum K*D | counts K | loss_sum 1] that ``vqvae._QuantizerBase._launch`` lays out contiguously;
     every rank then runs the identical finalize kernels on identical reduced values, so replicas stay
     bit-identical without a broadcast.  Loss and perplexity are those of the concatenated batch.
 
-Code sharding -- ``CodeShardedVectorQuantizerEMA``.
+Code sharding (K = 65536 codes over 8 GPUs) -- ``CodeShardedVectorQuantizerEMA``.
     Every rank holds K/G codes (rows [rank*K/G, (rank+1)*K/G) of ``_embedding.weight``, ``_ema_w``,
     ``_ema_cluster_size``) and sees ALL tokens.  Exchanges per call:
       1. all-reduce(min) of the packed int64 (distance, global index) keys [N] -- RCCL has no MINLOC; min of

@@ -1,7 +1,7 @@
 """Deterministic, platform-independent synthetic data for the VQ bottleneck.
 
 The golden fixtures under ``tests/golden/`` are produced in one container (where
-the reference imports) and checked on another (the GPU box, where it does not
+the reference imports) and checked on another (one with a GPU, where it does not
 exist).  Inputs therefore come from a generator whose output bits depend on
 nothing but (seed, stream, index): a 32-bit integer mixer evaluated in int64
 with every intermediate product kept below 2**63 (no reliance on wrap-around),
@@ -98,7 +98,7 @@ def uniform_int(n: int, high: int, seed: int, stream: int = 0, device="cpu") -> 
 
 
 def c1_activations(n: int, d: int, p: float, seed: int, stream: int = 7, device="cpu") -> torch.Tensor:
-    """C1 activation model: N(0,1) rows scaled to unit RMS (T5 final RMS-norm,
+    """C1 activation model : N(0,1) rows scaled to unit RMS (T5 final RMS-norm,
     python_transformers/modeling_t5.py:191-207,864), then inverted dropout with rate p (:865).
     The row RMS is taken from the exact integer sums, so the result is bit-reproducible."""
     a = _ih8(n * d, seed, stream, device).view(n, d)
@@ -112,7 +112,7 @@ def c1_activations(n: int, d: int, p: float, seed: int, stream: int = 7, device=
 
 
 def clustered(n: int, codebook: torch.Tensor, sigma: float, seed: int, stream: int = 11):
-    """x_i = W[c_i] + sigma * noise with c_i uniform over the codebook (SURVEY 8d 'uniform' regime).
+    """x_i = W[c_i] + sigma * noise with c_i uniform over the codebook ('uniform' regime).
     Returns (x [n, D] fp32, c [n] int64)."""
     k, d = codebook.shape
     c = uniform_int(n, k, seed, stream, codebook.device)

@@ -53,7 +53,7 @@ _EE_STATE = weakref.WeakKeyDictionary()
 # fp16 image of the codebook for the filtered search (ops.code_image), kept between calls like |e|^2 and under the same
 # key: (block, data_ptr, _version).  The kernel that writes the codebook (EMA update) writes its image too, a search that
 # finds no valid image makes it in the module's block instead of its own workspace -- either way the NEXT search's
-# preparation pass reads no codebook row (DESIGN.md section 8).  Only the base module's own flows keep one.
+# preparation pass reads no codebook row.  Only the base module's own flows keep one.
 _IMG_STATE = weakref.WeakKeyDictionary()
 
 
@@ -130,13 +130,13 @@ class _QuantizerBase(nn.Module):
     # -> all-reduce -> finalize, everything on one stream.  "overlap": the statistics pass runs first and alone, the
     # all-reduce of its head starts at once (async_op) and runs under the second pass, which writes the per-token
     # outputs (straight-through values, q - x, indices); finalize waits for it.  Same results; costs one more read of x
-    # ("overlap the all-reduce with K2").  bench.py --gpus N times both.
+    # (the all-reduce overlaps with the gather and loss pass).  bench.py --gpus N times both.
     stats_exchange = "serial"
 
     def __init__(self):
         super().__init__()
         # both libraries are loaded here, on the constructing thread: the first caller of a backward-only op is the
-        # autograd worker thread, and a dlopen (or a failing one, retried) must never happen there (DESIGN.md section 11)
+        # autograd worker thread, and a dlopen (or a failing one, retried) must never happen there
         _lib.load_all()
 
     def _flatten(self, inputs, srl):
@@ -176,7 +176,7 @@ class _QuantizerBase(nn.Module):
     deterministic = False
     # True: small problems (fewer than 256 tiles of 128 x 128, D % 256 == 0) without an EMA update -- evaluation, or the
     # plain variant -- take ONE launch (t5vq_vq_forward_small_f32): same results bit for bit.  Off by default: measured
-    # at C2 it runs level with the three-launch chain (45.0 against 45.7 us back to back; DESIGN.md section 3), so the
+    # at C2 it runs level with the three-launch chain (45.0 against 45.7 us back to back), so the
     # default stays the path with the longer record.
     small_forward = False
     index_mode = "reference"     # disentangled mode: "reference" = slice-relative indices used as rows (the
