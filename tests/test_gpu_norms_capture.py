@@ -127,3 +127,61 @@ def test_an_eager_graph_on_the_capturing_stream_is_no_obstacle():
         torch.cuda.synchronize()
         assert torch.equal(got, want)
     del living
+
+
+def test_captured_autograd_steps_draw_from_the_generator():
+    """No ticket: every replay draws anew, and its backward drops what its forward dropped."""
+    from t5vqvae_amd import norms
+    x, g = torch.ones(200, 768, device="cuda"), torch.ones(200, 768, device="cuda")
+    zero, one = torch.zeros(768, device="cuda"), torch.ones(768, device="cuda")
+
+    def step():
+        leaf, branch = x.detach().requires_grad_(True), x.detach().requires_grad_(True)
+        y = norms.dropout(leaf, 0.5)
+        total = norms.add_norm(torch.zeros_like(x), branch, zero, one, branch_p=0.5, p=0.5)
+        return (y.detach(), torch.autograd.grad(y, leaf, g)[0], total[1].detach(),
+                torch.autograd.grad(total[1], branch, g)[0])
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        res = step()
+    seen = []
+    for _ in range(4):
+        graph.replay()
+        torch.cuda.synchronize()
+        y, gx, total, gb = res
+        assert torch.equal(y, gx) and torch.equal(total, gb) and not torch.equal(y != 0, total != 0)
+        assert 0.45 < float((y != 0).float().mean()) < 0.55
+        assert not any(torch.equal(y, s) for s in seen)
+        seen.append(y.clone())
+        step()                                                    # the program's own eager draws in between
+
+
+def test_graphed_callables():
+    """torch captures a module's forward and backward into two graphs of its own: the same results as eager."""
+    from t5vqvae_amd import norms
+    class Layer(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.first, self.last = norms.Norm(96), norms.Norm(96, "rms")
+
+        def forward(self, h, br):
+            out, total = self.first(h, br)
+            return self.last(out) * 2.0 + total
+    h, br, g = rows(64, 96, 641), rows(64, 96, 642), rows(64, 96, 643)
+    layer = Layer().cuda()
+    with torch.no_grad():
+        for k, p in enumerate(layer.parameters()):
+            p.copy_(rows(1, 96, 644 + k)[0])
+
+    def step(f):
+        a, b = h.detach().requires_grad_(True), br.detach().requires_grad_(True)
+        y = f(a, b)
+        return (y.detach().clone(),) + tuple(t.clone() for t in torch.autograd.grad(y, [a, b, *layer.parameters()], g))
+    want = step(layer)
+    graphed = torch.cuda.make_graphed_callables(layer, (h.detach().requires_grad_(True), br.detach().requires_grad_(True)))
+    for _ in range(3):
+        for a, b in zip(step(graphed), want):
+            assert torch.equal(a, b)
+        torch.cuda.synchronize()

@@ -86,3 +86,24 @@ def test_tensors_that_stand_for_their_negative():
     assert torch._neg_view(h).is_neg()
     for a, c in zip(lazy, done):
         assert torch.equal(a, c)
+
+
+def test_inference_mode_and_saved_tensors_kept_elsewhere():
+    from t5vqvae_amd import norms
+    h, br, w, b, go, gs = tensors()
+    t = torch.tensor([3, 8], device="cuda")
+
+    def run():
+        return norms.add_norm(h, br, w, b, branch_p=0.2, p=0.1, ticket=t) + (norms.dropout(h, 0.3, br, ticket=t),)
+    plain = run()
+    with torch.inference_mode():
+        quiet = run()
+    assert all(torch.equal(a, c) for a, c in zip(plain, quiet))
+    grads = []
+    for away in (False, True):
+        leaves = [v.detach().requires_grad_(True) for v in (h, br, w, b)]
+        with torch.autograd.graph.save_on_cpu() if away else torch.autograd.graph.saved_tensors_hooks(lambda v: v, lambda v: v):
+            out, total = norms.add_norm(*leaves, branch_p=0.2, p=0.1, ticket=t)
+            y = norms.dropout(out, 0.3, total, ticket=t)
+        grads.append(torch.autograd.grad((y, total), leaves, (go, gs)))
+    assert all(torch.equal(a, c) for a, c in zip(*grads))
